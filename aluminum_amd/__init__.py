@@ -16,5 +16,5 @@ from .capi import (  # noqa: F401
     release_scratch, CHAIN_POLLS_NONE, planned_launches,
     ring_allreduce,
     ring_reduce_scatter, ring_allgather, halo_pack, halo_unpack, halo_face_elems,
-    fill, narrow_f32, widen_f32, copy, Flag, torch_dtype, dtype_size, check_op,
+    fill, narrow_f32, widen_f32, copy, rms_norm, rms_norm_grad, rms_norm_grad_workspace, TensorList, Flag, torch_dtype, dtype_size, check_op,
 )

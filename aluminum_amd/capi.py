@@ -98,6 +98,16 @@ def load():
     L.alamd_narrow_f32.argtypes = [vp, vp, sz, i, vp]
     L.alamd_widen_f32.argtypes = [vp, vp, sz, i, vp]
     L.alamd_copy.argtypes = [vp, vp, sz, vp]
+    fl = C.c_float
+    L.alamd_rms_norm.argtypes = [vp, sz, vp, vp, sz, pvp, i, sz, vp, i, vp, vp, sz, sz, sz, i, fl, vp]
+    L.alamd_rms_norm_grad_workspace.argtypes = [sz, sz]
+    L.alamd_rms_norm_grad_workspace.restype = sz
+    L.alamd_rms_norm_grad.argtypes = [vp, sz, pvp, i, sz, vp, sz, vp, sz, vp, vp, i, vp, sz, sz, i, vp, vp]
+    L.alamd_tensor_list_create.argtypes = [pvp, pvp, pvp, C.POINTER(sz), C.POINTER(i), sz]
+    L.alamd_tensor_list_destroy.argtypes = [vp]
+    L.alamd_global_norm.argtypes = [vp, vp, vp, vp]
+    L.alamd_clip_to_norm.argtypes = [vp, vp, fl, fl, vp]
+    L.alamd_clip_global_norm.argtypes = [vp, vp, fl, fl, vp, vp]
     _lib = L
     return L
 
@@ -345,6 +355,177 @@ def copy(dst, src, nbytes=None, stream=None):
     nbytes = src.numel() * src.element_size() if nbytes is None else nbytes
     _check(load().alamd_copy(C.c_void_p(dst.data_ptr()), C.c_void_p(src.data_ptr()), nbytes,
                              _stream(stream)))
+
+
+def _on_device(t):
+    import torch
+    if not t.is_cuda:
+        raise AlError(1, "buffers must live on the GPU")
+    if t.get_device() != torch.cuda.current_device():
+        raise AlError(1, "a buffer lives on device %d, the current device is %d" % (t.get_device(), torch.cuda.current_device()))
+
+
+def _matrix(t, shape, dtype, what):
+    """(address, elements between rows) of a matrix on the GPU whose rows are contiguous."""
+    if t.shape != shape or t.dtype != dtype:
+        raise AlError(1, "%s is %s of %s, expected %s of %s" % (what, tuple(t.shape), t.dtype, tuple(shape), dtype))
+    _on_device(t)
+    row, col = t.stride()
+    if col != 1 and shape[1] > 1:
+        raise AlError(1, "rows must be contiguous")
+    return t.data_ptr(), (row if shape[0] > 1 else max(row, shape[1]))
+
+
+def _vector(t, n, dtype, what):
+    """Address of n contiguous elements on the GPU, of any shape."""
+    if t.numel() != n or t.dtype != dtype:
+        raise AlError(1, "%s has %d elements of %s, expected %d of %s" % (what, t.numel(), t.dtype, n, dtype))
+    _on_device(t)
+    if not t.is_contiguous():
+        raise AlError(1, "buffers must be contiguous")
+    return t.data_ptr()
+
+
+def _rank_matrices(tensors, shape, dtype, what):
+    """Table of the ranks' matrices, which share one distance between rows, and that distance."""
+    arr = (C.c_void_p * len(tensors))()
+    stride = None
+    for k, t in enumerate(tensors):
+        arr[k], s = _matrix(t, shape, dtype, what)
+        if stride is not None and s != stride:
+            raise AlError(1, "%s of every rank must have the same distance between rows" % what)
+        stride = s
+    return arr, stride
+
+
+def rms_norm(out, ins, weight=None, residual=None, sum_out=None, rstd=None, scales=None, group=0, eps=1e-6, stream=None):
+    """out = rms norm of ins[0] + .. + ins[P-1] (+ residual), times weight (alamd_rms_norm).  All matrices are
+    [rows, cols] with contiguous rows; `sum_out` receives the sum, `rstd` (fp32, [rows]) what rms_norm_grad needs.
+    With `scales` (fp32, [rows, groups]) out is torch.float8_e4m3fn in groups of `group` columns (0: a row)."""
+    import torch
+    x = ins[0]
+    if x.dim() != 2:
+        raise AlError(1, "rms_norm takes matrices of [rows, cols]")
+    shape, dtype = x.shape, x.dtype
+    rows, cols = shape
+    table, in_stride = _rank_matrices(ins, shape, dtype, "a rank's input")
+    out_p, out_stride = _matrix(out, shape, dtype if scales is None else torch.float8_e4m3fn, "out")
+    res_p = sum_p = None
+    res_stride = 0
+    if residual is not None:
+        res_p, res_stride = _matrix(residual, shape, dtype, "residual")
+    if sum_out is not None:
+        sum_p, s = _matrix(sum_out, shape, dtype, "sum_out")
+        if residual is not None and s != res_stride:
+            raise AlError(1, "residual and sum_out must have the same distance between rows")
+        res_stride = s
+    w_p, w_dt = _weight(weight, cols, dtype)
+    groups = -(-cols // group) if group > 0 else 1
+    _check(load().alamd_rms_norm(
+        out_p, out_stride, sum_p, res_p, res_stride, table, len(ins), in_stride, w_p, w_dt,
+        None if rstd is None else _vector(rstd, rows, torch.float32, "rstd"),
+        None if scales is None else _vector(scales, rows * groups, torch.float32, "scales"),
+        group, rows, cols, DTYPES.index(_infer_dtype(x)), eps, _stream(stream)))
+
+
+def _weight(weight, cols, dtype):
+    import torch
+    if weight is None:
+        return None, DTYPES.index("f32")
+    if weight.dtype != dtype and weight.dtype != torch.float32:
+        raise AlError(3, "the weight has the rows' type or float32, not %s" % weight.dtype)
+    return _vector(weight, cols, weight.dtype, "weight"), DTYPES.index(_infer_dtype(weight))
+
+
+def rms_norm_grad_workspace(rows, cols):
+    """Bytes of device memory that rms_norm_grad needs for dweight (alamd_rms_norm_grad_workspace)."""
+    return load().alamd_rms_norm_grad_workspace(rows, cols)
+
+
+def rms_norm_grad(dx, dys, x, rstd, weight=None, dsum=None, dweight=None, workspace=None, stream=None):
+    """Backward pass of rms_norm (alamd_rms_norm_grad): dx (may be None) from the ranks' gradients dys of the
+    output and dsum of the sum; dweight (may be None) has the weight's type, or without a weight any that a weight
+    may have.  `workspace`: a contiguous tensor of at least rms_norm_grad_workspace(rows, cols) bytes."""
+    import torch
+    if x.dim() != 2:
+        raise AlError(1, "rms_norm_grad takes matrices of [rows, cols]")
+    shape, dtype = x.shape, x.dtype
+    rows, cols = shape
+    table, dy_stride = _rank_matrices(dys, shape, dtype, "a rank's gradient")
+    x_p, x_stride = _matrix(x, shape, dtype, "x")
+    dx_p, dx_stride = (None, cols) if dx is None else _matrix(dx, shape, dtype, "dx")
+    ds_p, ds_stride = (None, cols) if dsum is None else _matrix(dsum, shape, dtype, "dsum")
+    w_p, w_dt = _weight(weight, cols, dtype)
+    dw_p = ws_p = None
+    if dweight is not None:
+        if weight is None:
+            w_dt = _weight(dweight, cols, dtype)[1]
+        dw_p = _vector(dweight, cols, dweight.dtype if weight is None else weight.dtype, "dweight")
+        if rows:
+            need = rms_norm_grad_workspace(rows, cols)
+            have = 0 if workspace is None else workspace.numel() * workspace.element_size()
+            if have < need:
+                raise AlError(1, "dweight needs a workspace of %d bytes, not %d" % (need, have))
+            ws_p = _vector(workspace, workspace.numel(), workspace.dtype, "workspace")
+    _check(load().alamd_rms_norm_grad(
+        dx_p, dx_stride, table, len(dys), dy_stride, x_p, x_stride, ds_p, ds_stride,
+        _vector(rstd, rows, torch.float32, "rstd"), w_p, w_dt, dw_p, rows, cols, DTYPES.index(_infer_dtype(x)), ws_p,
+        _stream(stream)))
+
+
+class TensorList:
+    """A list of buffers (alamd_tensor_list): the gradients `ins` of float16, bfloat16 and float32, clipped into `outs`
+    or in place.  Holds its tensors, and a workspace of its own for calls that are given none; such calls have to
+    follow one another."""
+
+    WORKSPACE_BYTES = 16384
+
+    def __init__(self, ins, outs=None):
+        import torch
+        self._h = C.c_void_p(None)
+        self._keep = (list(ins), None if outs is None else list(outs))
+        n = len(self._keep[0])
+        for t in self._keep[0] + (self._keep[1] or []):
+            _on_device(t)
+        if outs is not None:
+            if len(self._keep[1]) != n:
+                raise AlError(1, "%d outputs for %d tensors" % (len(self._keep[1]), n))
+            for k, (a, b) in enumerate(zip(*self._keep)):
+                if a.numel() != b.numel() or a.dtype != b.dtype:
+                    raise AlError(1, "output %d is not like its tensor" % k)
+        counts = (C.c_size_t * n)(*[t.numel() for t in self._keep[0]])
+        dtypes = (C.c_int * n)(*[DTYPES.index(_infer_dtype(t)) for t in self._keep[0]])
+        _check(load().alamd_tensor_list_create(C.byref(self._h), None if outs is None else _table(self._keep[1]),
+                                               _table(self._keep[0]), counts, dtypes, n))
+        self._workspace = torch.empty(self.WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+
+    def _space(self, workspace):
+        w = self._workspace if workspace is None else workspace
+        if w.numel() * w.element_size() < self.WORKSPACE_BYTES:
+            raise AlError(1, "the workspace has less than %d bytes" % self.WORKSPACE_BYTES)
+        return _vector(w, w.numel(), w.dtype, "workspace")
+
+    def global_norm(self, norm, workspace=None, stream=None):
+        """norm[0] = the norm over all elements (alamd_global_norm)."""
+        import torch
+        _check(load().alamd_global_norm(self._h, _vector(norm, 1, torch.float32, "norm"), self._space(workspace),
+                                        _stream(stream)))
+
+    def clip_to_norm(self, norm, max_norm, eps=1e-6, stream=None):
+        """Scales by max_norm / (norm[0] + eps) where that is below 1 (alamd_clip_to_norm)."""
+        import torch
+        _check(load().alamd_clip_to_norm(self._h, _vector(norm, 1, torch.float32, "norm"), max_norm, eps, _stream(stream)))
+
+    def clip_global_norm(self, norm, max_norm, eps=1e-6, workspace=None, stream=None):
+        """Both (alamd_clip_global_norm)."""
+        import torch
+        _check(load().alamd_clip_global_norm(self._h, _vector(norm, 1, torch.float32, "norm"), max_norm, eps,
+                                             self._space(workspace), _stream(stream)))
+
+    def destroy(self):
+        if self._h:
+            h, self._h = self._h, C.c_void_p(None)
+            _check(load().alamd_tensor_list_destroy(h))
 
 
 class Flag:

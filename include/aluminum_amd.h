@@ -407,6 +407,103 @@ int alamd_flag_timed_out(alamd_flag *flag);
  * readings of the other kernels are scaled by. */
 int alamd_copy(void *dst, const void *src, size_t bytes, void *stream);
 
+/* ---- root-mean-square norm behind a sum over ranks ----------------------- */
+
+/* What a layer split over P logical ranks does with its partial results: they
+ * are summed (the Allreduce), the residual stream is added, and the sum is
+ * normalised for the next product - in the one pass that folds the ranks.  For
+ * every row of `cols` elements
+ *   s    = ins[0] + ins[1] + .. + ins[P-1] (+ residual)
+ *   rstd = 1 / sqrt(sum(s * s) / cols + eps)
+ *   out  = s * weight * rstd
+ * in fp32; `out` and `sum` (s itself, the residual stream of the next layer)
+ * are each rounded once, to nearest.  P = 1 is the plain operator.  The fold
+ * is not one of the named orders of alamd_combine: s is not rounded between
+ * the ranks, so with 16-bit rows it is nearer to the sum than any of them and
+ * `sum` need not have the bits that alamd_combine gives.  The reference, a
+ * communication library, has no counterpart.
+ *   dtype: ALAMD_F16, ALAMD_BF16 or ALAMD_F32, the type of ins, residual, sum
+ *     and (without scales) out.  weight: cols elements of that type or of fp32
+ *     (weight_dtype), or NULL for ones.
+ *   Strides are in elements between the starts of rows (>= cols): in_stride of
+ *     every ins, residual_stride of residual and sum, out_stride of out.
+ *   residual, sum, rstd (one fp32 per row, what the backward pass needs) may be
+ *     NULL.
+ *   scales given: out is 8 bits an element, e4m3 (largest value 448), in groups of
+ *     `group` = 32, 64 or 128 columns (a row's last group may be shorter), or of
+ *     the whole row (group = 0).  scales[row * groups + g] = max(max|y| / 448,
+ *     2^-126) over the group, y as above before rounding, and out = y / scale
+ *     rounded to nearest: out * scale stands for y.  An infinity in a group makes its
+ *     scale infinite and itself NaN, a NaN makes the group NaN.
+ * `sum` and `out` may each take the place of an input or of the residual (the
+ * same address and stride, and for `out` no scales); other overlaps are
+ * ALAMD_ERR_OVERLAP.  cols is at most ALAMD_RMS_NORM_MAX_COLS.  Nothing is done
+ * for rows = 0 or cols = 0.  A result depends on the values alone, not on the
+ * stream, the rows around it or the run. */
+#define ALAMD_RMS_NORM_MAX_COLS 32768
+int alamd_rms_norm(void *out, size_t out_stride, void *sum, const void *residual,
+                   size_t residual_stride, const void *const *ins, int P, size_t in_stride,
+                   const void *weight, int weight_dtype, float *rstd, float *scales,
+                   size_t group, size_t rows, size_t cols, int dtype, float eps,
+                   void *stream);
+
+/* Its backward pass.  With x the `sum` of the forward pass (the input itself if
+ * P = 1 and there was no residual), rstd what it wrote, dys[r] the gradient of
+ * `out` that rank r holds and dsum the gradient that reaches `sum` on its way
+ * to the next layer (NULL: none):
+ *   dy = dys[0] + .. + dys[P-1],  n = x * rstd,  g = dy * weight
+ *   dx = rstd * (g - n * sum(g * n) / cols) (+ dsum)
+ *   dweight = sum over the rows of dy * n
+ * in fp32, each rounded once.  dx is the gradient of `sum`, hence of every
+ * rank's input and of the residual.  dweight has weight_dtype; it is written
+ * (zeros for rows = 0), not added to, and the order of its additions depends on
+ * the sizes alone.  dx or dweight may be NULL; dweight needs `workspace`, device
+ * memory of alamd_rms_norm_grad_workspace(rows, cols) bytes that no call running
+ * at the same time uses.  dx may take the place of one of dys, x or dsum (same
+ * address and stride). */
+size_t alamd_rms_norm_grad_workspace(size_t rows, size_t cols);
+int alamd_rms_norm_grad(void *dx, size_t dx_stride, const void *const *dys, int P,
+                        size_t dy_stride, const void *x, size_t x_stride, const void *dsum,
+                        size_t dsum_stride, const float *rstd, const void *weight,
+                        int weight_dtype, void *dweight, size_t rows, size_t cols, int dtype,
+                        void *workspace, void *stream);
+
+/* ---- norm and clipping over many buffers ---------------------------------- */
+
+/* A list of n buffers - the gradients of a model after their Allreduce -,
+ * ins[t] of counts[t] elements of dtypes[t] (ALAMD_F16, ALAMD_BF16, ALAMD_F32,
+ * mixed as they come), and where they go when they are clipped: outs[t], or in
+ * place where outs is NULL or outs[t] == ins[t].  No other overlap of what is
+ * written with anything is taken (ALAMD_ERR_OVERLAP): a buffer can be in a list once.
+ * A set-up call: it allocates device memory for the table and returns when that
+ * is filled.  The list holds the addresses; it belongs to the current device,
+ * and the buffers stay the caller's and have to outlive its use, as the list has
+ * to outlive every graph that holds a call with it.  Destroying it waits for the
+ * device. */
+typedef struct alamd_tensor_list alamd_tensor_list;
+int alamd_tensor_list_create(alamd_tensor_list **list, void *const *outs, const void *const *ins,
+                             const size_t *counts, const int *dtypes, size_t n);
+int alamd_tensor_list_destroy(alamd_tensor_list *list);
+
+/* *norm (fp32, device memory) = sqrt of the sum of the squares of every element
+ * of the list, squared and summed in fp64 in an order that depends on the list
+ * alone; 0 for an empty list.  `workspace`: ALAMD_GLOBAL_NORM_WORKSPACE_BYTES of
+ * device memory, aligned to 8 bytes, that no call running at the same time uses. */
+#define ALAMD_GLOBAL_NORM_WORKSPACE_BYTES 16384
+int alamd_global_norm(const alamd_tensor_list *list, float *norm, void *workspace, void *stream);
+
+/* outs[t] = ins[t] * factor for every buffer of the list, with
+ *   factor = 1 if *norm + eps <= max_norm, else max_norm / (*norm + eps)
+ * in fp32, the product rounded once.  *norm is read on the device: what
+ * alamd_global_norm wrote there, or the norm over more than this list.  A norm that is
+ * NaN makes everything NaN; buffers that stay in place are left alone where the factor is 1. */
+int alamd_clip_to_norm(const alamd_tensor_list *list, const float *norm, float max_norm, float eps,
+                       void *stream);
+
+/* Both: the norm of the list, and the list clipped to it. */
+int alamd_clip_global_norm(const alamd_tensor_list *list, float *norm, float max_norm, float eps,
+                           void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
