@@ -86,70 +86,75 @@ __device__ __forceinline__ uint32_t group_max(uint32_t x, unsigned lanes) {
   return x;
 }
 
-// `lds`: a word for each wave of the workgroup.  A caller that comes back needs another one the next time
-// and may use the first again the time after (a wave that writes there has met all others since).
+// The waves of a workgroup of up to 1024 threads meet in `lds`, kWaves * words floats.  A caller that comes back
+// needs another place the next time and may use the first again the time after (a wave that writes there has
+// met all others since).
+constexpr int kWaves = 16;
 template <int TEAM> __device__ __forceinline__ float team_sum(float x, float *lds) {
-  if constexpr (TEAM <= 64) return lanes_sum<TEAM>(x);
-  constexpr int WAVES = TEAM / 64;
-  x = lanes_sum<64>(x);
-  const unsigned wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63u) == 0) lds[wave] = x;
-  __syncthreads();
-  const float *first = lds + wave / WAVES * WAVES;
-  x = first[0];
-#pragma unroll
-  for (int k = 1; k < WAVES; ++k) x += first[k];
+  x = lanes_sum<(TEAM ? TEAM : 64)>(x);
+  if constexpr (TEAM == 0) {
+    const unsigned waves = blockDim.x >> 6;
+    if (waves == 1) return x;
+    if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = lds[0];
+    for (unsigned k = 1; k < waves; ++k) x += lds[k];
+  }
   return x;
 }
-// A sum and a largest word in one meeting; `lds`: two words for each wave.
+// A sum and a largest word in one meeting.
 template <int TEAM> __device__ __forceinline__ void team_sum_max(float &x, uint32_t &m, float *lds) {
-  x = lanes_sum<(TEAM < 64 ? TEAM : 64)>(x);
-  m = group_max(m, TEAM < 64 ? TEAM : 64);
-  if constexpr (TEAM > 64) {
-    constexpr int WAVES = TEAM / 64;
-    const unsigned wave = threadIdx.x >> 6;
+  x = lanes_sum<(TEAM ? TEAM : 64)>(x);
+  m = group_max(m, TEAM ? TEAM : 64);
+  if constexpr (TEAM == 0) {
+    const unsigned waves = blockDim.x >> 6;
+    if (waves == 1) return;
     if ((threadIdx.x & 63u) == 0) {
-      lds[2 * wave] = x;
-      lds[2 * wave + 1] = __uint_as_float(m);
+      lds[2 * (threadIdx.x >> 6)] = x;
+      lds[2 * (threadIdx.x >> 6) + 1] = __uint_as_float(m);
     }
     __syncthreads();
-    const float *first = lds + wave / WAVES * WAVES * 2;
-    x = first[0];
-    m = __float_as_uint(first[1]);
-#pragma unroll
-    for (int k = 1; k < WAVES; ++k) {
-      x += first[2 * k];
-      m = umax(m, __float_as_uint(first[2 * k + 1]));
+    x = lds[0];
+    m = __float_as_uint(lds[1]);
+    for (unsigned k = 1; k < waves; ++k) {
+      x += lds[2 * k];
+      m = umax(m, __float_as_uint(lds[2 * k + 1]));
     }
   }
 }
 
 // ---- a row in registers -------------------------------------------------------
 
-// Lane l of a team holds the vectors l, TEAM + l, 2 TEAM + l, ..: vector i covers the elements [i * VE, ..) of the
-// row.  Where the row does not end with a whole vector, the last one is moved back to end with it: its first
-// `skip` elements are then the lane's before it too.  cols >= VE.
+// A team is the whole workgroup (TEAM = 0: as many waves as the row needs) or one of its waves (64).  Lane l of
+// a team of n lanes holds the vectors l, n + l, 2 n + l, ..: vector i covers the elements [i * VE, ..) of the row.
+// Where the row does not end with a whole vector, the last one is moved back to end with it: its first `skip`
+// elements are then the lane's before it too.  cols >= VE.
 template <typename T, int TEAM, int NV> struct RowTeam {
-  static_assert(TEAM >= 64, "a wave's lanes belong to one row");
+  static_assert(TEAM == 0 || TEAM == 64, "a wave's lanes belong to one row");
   static constexpr int VE = Row<T>::VE;
   static constexpr unsigned kNowhere = 0x7ffffff0u;  // an offset behind every row
-  unsigned lane, index;
+  unsigned lane, index, size;
   unsigned cols;
+  bool ragged;        // the last vector was moved back
   unsigned off[NV];   // byte offset in the row of the lane's vectors
   unsigned skip[NV];  // elements of each that another lane counts
 
   __device__ __forceinline__ explicit RowTeam(unsigned n) : cols(n) {
-    lane = threadIdx.x % TEAM;
-    index = (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / TEAM));
+    size = TEAM ? (unsigned)TEAM : blockDim.x;
+    lane = TEAM ? threadIdx.x % 64u : threadIdx.x;
+    index = TEAM ? (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64u)) : 0u;
     const unsigned full = n / VE, rem = n % VE;
+    ragged = rem != 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const unsigned i = (unsigned)v * TEAM + lane;
-      const bool last = rem && i == full;
+      const unsigned i = (unsigned)v * size + lane;
+      const bool last = ragged && i == full;
       off[v] = i < full ? i * 16u : last ? (n - VE) * (unsigned)sizeof(T) : kNowhere;
       skip[v] = last ? VE - rem : 0u;
     }
   }
+  // The first element of vector v, counted as if every vector were in its place.
+  __device__ __forceinline__ unsigned element(int v) const { return ((unsigned)v * size + lane) * VE; }
   // Whether element j of vector v is this lane's to count (elements of no row are zeros and may be counted).
   __device__ __forceinline__ bool counts(int v, int j) const { return (unsigned)j >= skip[v]; }
 
@@ -161,13 +166,13 @@ template <typename T, int TEAM, int NV> struct RowTeam {
                                        bool live) const {
     const auto r = rsrc(base, pitch, row, live, cols * (unsigned)sizeof(T));
 #pragma unroll
-    for (int v = 0; v < NV; ++v) raw[v] = __builtin_amdgcn_raw_buffer_load_b128(r, off[v], 0, 0);
+    for (int v = 0; v < NV; ++v) raw[v] = __builtin_amdgcn_raw_buffer_load_b128(r, off[v], 0, kAuxLoadStream);
   }
   __device__ __forceinline__ void store(const u32x4 (&raw)[NV], char *base, unsigned long long pitch, unsigned long long row,
                                         bool live) const {
     const auto r = rsrc(base, pitch, row, live, cols * (unsigned)sizeof(T));
 #pragma unroll
-    for (int v = 0; v < NV; ++v) __builtin_amdgcn_raw_buffer_store_b128(raw[v], r, off[v], 0, 0);
+    for (int v = 0; v < NV; ++v) __builtin_amdgcn_raw_buffer_store_b128(raw[v], r, off[v], 0, kAuxStoreStream);
   }
   __device__ __forceinline__ void load_weight(float (&w)[VE], int v, const char *weight, int w32) const {
     if constexpr (!std::is_same<T, float>::value) {
@@ -197,16 +202,16 @@ template <typename T, int TEAM, int NV> struct RowTeam {
       q[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * by, x[4 * j + 3] * by, lo, true);
     }
     const unsigned at = off[v] / (unsigned)sizeof(T);
-    if (skip[v] == 0) {
-      const auto r = rsrc(base, pitch, row, live, cols);
-      if constexpr (VE == 8) {
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        const u32x2 both = {q[0], q[1]};
-        __builtin_amdgcn_raw_buffer_store_b64(both, r, at, 0, 0);
-      } else {
-        __builtin_amdgcn_raw_buffer_store_b32(q[0], r, at, 0, 0);
-      }
-    } else if (live) {
+    const unsigned whole = ragged && skip[v] ? kNowhere : at;
+    const auto r = rsrc(base, pitch, row, live, cols);
+    if constexpr (VE == 8) {
+      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+      const u32x2 both = {q[0], q[1]};
+      __builtin_amdgcn_raw_buffer_store_b64(both, r, whole, 0, kAuxStoreStream);
+    } else {
+      __builtin_amdgcn_raw_buffer_store_b32(q[0], r, whole, 0, kAuxStoreStream);
+    }
+    if (ragged && skip[v] && live) {
       char *o = base + row * pitch + at;
 #pragma unroll
       for (int j = 1; j < VE; ++j)

@@ -46,54 +46,78 @@ enum { OUT_SAME = 0, OUT_E4M3_ROW = 1, OUT_E4M3_GROUP = 2 };
 // its reciprocal is finite whatever a is.
 constexpr float kE4m3Max = 448.0f, kLeastScale = 1.17549435e-38f;
 __device__ __forceinline__ float scale_of(unsigned amax_bits) {
-  const float a = __uint_as_float(amax_bits) / kE4m3Max;
+  const float a = __uint_as_float(amax_bits) * (1.0f / kE4m3Max);
   return a < kLeastScale ? kLeastScale : a;  // a NaN passes
 }
 
+// Streams whose loads are issued together: eight vectors a lane.
+template <int NV> constexpr int streams_at_once() { return NV >= 8 ? 1 : 8 / NV > 4 ? 4 : 8 / NV; }
+
+// The sum of P streams of a row, in rank order.
+template <int B, typename Team, typename T, int NV, int VE>
+__device__ __forceinline__ void sum_streams(float (&s)[NV][VE], const Team &team, const char *const *in, int P,
+                                            unsigned long long pitch, unsigned long long row, bool live) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int j = 0; j < VE; ++j) s[v][j] = -0.0f;  // -0 + x is x, whatever x
+  for (int k = 0; k < P; k += B) {
+    u32x4 raw[B][NV];
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (k + b < P) team.load(raw[b], in[k + b], pitch, row, live);
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (k + b < P) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          float x[VE];
+          Row<T>::unpack(x, raw[b][v]);
+#pragma unroll
+          for (int j = 0; j < VE; ++j) s[v][j] += x[j];
+        }
+      }
+  }
+}
+
+constexpr int kWaveTeams = 4;  // rows, one a wave, of a workgroup whose teams are waves
+
 template <typename T, int TEAM, int NV, int OUT>
-__global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) rms_norm_kernel(const NormParams p) {
+__global__ void __launch_bounds__(TEAM ? 64 * kWaveTeams : 1024) rms_norm_kernel(const NormParams p) {
   constexpr int VE = Row<T>::VE;
-  constexpr int THREADS = TEAM < 256 ? 256 : TEAM;
-  constexpr int TEAMS = THREADS / TEAM;
-  __shared__ float lds[2][THREADS / 64 * 2];
+  constexpr int TEAMS = TEAM ? kWaveTeams : 1;
+  __shared__ float lds[2][kWaves * 2];
   const RowTeam<T, TEAM, NV> team(p.cols);
   int turn = 0;
   for (unsigned long long r0 = (unsigned long long)blockIdx.x * TEAMS; r0 < p.rows;
        r0 += (unsigned long long)gridDim.x * TEAMS, turn ^= 1) {
     const unsigned long long row = r0 + team.index;
     const bool live = row < p.rows;
+    u32x4 res[NV];
+    if (p.res) team.load(res, p.res, p.res_pitch, row, live);
     float s[NV][VE];
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int j = 0; j < VE; ++j) s[v][j] = 0.0f;
-    for (int k = 0; k < p.P; ++k) {
-      u32x4 raw[NV];
-      team.load(raw, p.in[k], p.in_pitch, row, live);
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        float x[VE];
-        Row<T>::unpack(x, raw[v]);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) s[v][j] = k == 0 ? x[j] : s[v][j] + x[j];
-      }
-    }
+    sum_streams<streams_at_once<NV>(), RowTeam<T, TEAM, NV>, T>(s, team, p.in, p.P, p.in_pitch, row, live);
     if (p.res) {
-      u32x4 raw[NV];
-      team.load(raw, p.res, p.res_pitch, row, live);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         float x[VE];
-        Row<T>::unpack(x, raw[v]);
+        Row<T>::unpack(x, res[v]);
 #pragma unroll
         for (int j = 0; j < VE; ++j) s[v][j] += x[j];
       }
     }
     float ss = 0.0f;
+    if (team.ragged) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+      for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int j = 0; j < VE; ++j) ss = fmaf(s[v][j], team.counts(v, j) ? s[v][j] : 0.0f, ss);
+        for (int j = 0; j < VE; ++j) ss = fmaf(s[v][j], team.counts(v, j) ? s[v][j] : 0.0f, ss);
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < VE; ++j) ss = fmaf(s[v][j], s[v][j], ss);
+    }
     u32x4 sum[NV];
     if (p.sum) {
 #pragma unroll
@@ -114,13 +138,11 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) rms_norm_kernel(const
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          const unsigned b = __float_as_uint(s[v][j]) & 0x7fffffffu;
-          am = b > am ? b : am;
-        }
+        for (int j = 0; j < VE; ++j) am = umax(am, __float_as_uint(s[v][j]) & 0x7fffffffu);
+      team_sum_max<TEAM>(ss, am, lds[turn]);
+    } else {
+      ss = team_sum<TEAM>(ss, lds[turn]);
     }
-    if constexpr (OUT == OUT_E4M3_ROW) team_sum_max<TEAM>(ss, am, lds[turn]);
-    else ss = team_sum<TEAM>(ss, lds[turn]);
     // The team has met: every lane has read its part of the row.  Nothing is written before, because a vector
     // that was moved back reads what another lane writes where the sum takes the residual's place.
     if (p.sum) team.store(sum, p.sum, p.res_pitch, row, live);
@@ -131,10 +153,9 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) rms_norm_kernel(const
 #pragma unroll
       for (int j = 0; j < VE; ++j) s[v][j] *= rstd;
     if constexpr (OUT == OUT_SAME) {
-      u32x4 raw[NV];
 #pragma unroll
-      for (int v = 0; v < NV; ++v) raw[v] = Row<T>::pack(s[v]);
-      team.store(raw, p.out, p.out_pitch, row, live);
+      for (int v = 0; v < NV; ++v) sum[v] = Row<T>::pack(s[v]);
+      team.store(sum, p.out, p.out_pitch, row, live);
     } else {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
@@ -145,16 +166,14 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) rms_norm_kernel(const
         } else {
           unsigned a = 0;
 #pragma unroll
-          for (int j = 0; j < VE; ++j) {
-            const unsigned b = __float_as_uint(s[v][j]) & 0x7fffffffu;
-            a = team.counts(v, j) && b > a ? b : a;
-          }
+          for (int j = 0; j < VE; ++j) a = umax(a, team.counts(v, j) ? __float_as_uint(s[v][j]) & 0x7fffffffu : 0u);
           a = group_max(a, (1u << p.group_log2) / VE);
           scale = scale_of(a);
-          const unsigned e = ((unsigned)v * TEAM + team.lane) * VE;
-          if (live && e < p.cols && (e & ((1u << p.group_log2) - 1)) == 0) p.scales[row * p.groups + (e >> p.group_log2)] = scale;
+          const unsigned e = team.element(v);
+          if (live && e < p.cols && (e & ((1u << p.group_log2) - 1)) == 0)
+            p.scales[row * p.groups + (e >> p.group_log2)] = scale;
         }
-        team.store_e4m3(s[v], v, 1.0f / scale, p.out, p.out_pitch, row, live);
+        team.store_e4m3(s[v], v, __builtin_amdgcn_rcpf(scale), p.out, p.out_pitch, row, live);
       }
     }
   }
@@ -214,11 +233,10 @@ struct GradParams {
 };
 
 template <typename T, int TEAM, int NV>
-__global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) rms_norm_grad_kernel(const GradParams p) {
+__global__ void __launch_bounds__(TEAM ? 64 * kWaveTeams : 1024) rms_norm_grad_kernel(const GradParams p) {
   constexpr int VE = Row<T>::VE;
-  constexpr int THREADS = TEAM < 256 ? 256 : TEAM;
-  constexpr int TEAMS = THREADS / TEAM;
-  __shared__ float lds[2][THREADS / 64 * 2];
+  constexpr int TEAMS = TEAM ? kWaveTeams : 1;
+  __shared__ float lds[2][kWaves];
   const RowTeam<T, TEAM, NV> team(p.cols);
   float dw[NV][VE];
 #pragma unroll
@@ -235,21 +253,7 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) rms_norm_grad_kernel(
     if (p.dsum) team.load(ds, p.dsum, p.dsum_pitch, row, live);
     const float rstd = live ? p.rstd[row] : 0.0f;
     float g[NV][VE];
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int j = 0; j < VE; ++j) g[v][j] = 0.0f;
-    for (int k = 0; k < p.P; ++k) {
-      u32x4 raw[NV];
-      team.load(raw, p.dy[k], p.dy_pitch, row, live);
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        float d[VE];
-        Row<T>::unpack(d, raw[v]);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) g[v][j] = k == 0 ? d[j] : g[v][j] + d[j];
-      }
-    }
+    sum_streams<streams_at_once<NV>(), RowTeam<T, TEAM, NV>, T>(g, team, p.dy, p.P, p.dy_pitch, row, live);
     float dot = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -284,10 +288,9 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) rms_norm_grad_kernel(
           for (int j = 0; j < VE; ++j) g[v][j] += d[j];
         }
       }
-      u32x4 raw[NV];
 #pragma unroll
-      for (int v = 0; v < NV; ++v) raw[v] = Row<T>::pack(g[v]);
-      team.store(raw, p.dx, p.dx_pitch, row, live);
+      for (int v = 0; v < NV; ++v) ds[v] = Row<T>::pack(g[v]);
+      team.store(ds, p.dx, p.dx_pitch, row, live);
     }
   }
   if (!p.partial) return;
@@ -437,17 +440,19 @@ int check_common(int P, size_t cols, int dtype, const void *weight, int weight_d
 constexpr size_t kMaxGrid = (size_t)1 << 21;
 
 template <typename T, int TEAM, int NV>
-int launch_norm(const NormParams &p, int out, hipStream_t stream) {
-  constexpr int THREADS = TEAM < 256 ? 256 : TEAM;
-  constexpr size_t TEAMS = THREADS / TEAM;
+int launch_norm(const NormParams &p, int out, unsigned threads, hipStream_t stream) {
+  constexpr size_t TEAMS = TEAM ? kWaveTeams : 1;
   size_t grid = (p.rows + TEAMS - 1) / TEAMS;
   if (grid > kMaxGrid) grid = kMaxGrid;
   auto kern = out == OUT_SAME ? rms_norm_kernel<T, TEAM, NV, OUT_SAME>
               : out == OUT_E4M3_ROW ? rms_norm_kernel<T, TEAM, NV, OUT_E4M3_ROW> : rms_norm_kernel<T, TEAM, NV, OUT_E4M3_GROUP>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(THREADS), 0, stream, p);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(threads), 0, stream, p);
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
+
+// Threads of a workgroup that holds a row of `need` vectors, nv of them a lane.
+inline unsigned row_threads(unsigned need, unsigned nv) { return ((need + nv - 1) / nv + 63u) & ~63u; }
 
 template <typename T> int norm_rows(const NormParams &p, int out, hipStream_t stream) {
   constexpr unsigned VE = Row<T>::VE;
@@ -460,27 +465,24 @@ template <typename T> int norm_rows(const NormParams &p, int out, hipStream_t st
     return ALAMD_OK;
   }
   const unsigned need = (p.cols + VE - 1) / VE;  // vectors of a row
-  if (need <= 64) return launch_norm<T, 64, 1>(p, out, stream);
-  if (need <= 256) return launch_norm<T, 256, 1>(p, out, stream);
-  if (need <= 512) return launch_norm<T, 256, 2>(p, out, stream);
-  if (need <= 1024) return launch_norm<T, 256, 4>(p, out, stream);
-  if (need <= 2048) return launch_norm<T, 1024, 2>(p, out, stream);
-  if (need <= 4096) return launch_norm<T, 1024, 4>(p, out, stream);
-  if constexpr (VE == 4) return launch_norm<T, 1024, 8>(p, out, stream);
+  if (need <= 64) return launch_norm<T, 64, 1>(p, out, 64 * kWaveTeams, stream);
+  if (need <= 128) return launch_norm<T, 64, 2>(p, out, 64 * kWaveTeams, stream);
+  if (need <= 2048) return launch_norm<T, 0, 2>(p, out, row_threads(need, 2), stream);
+  if (need <= 4096) return launch_norm<T, 0, 4>(p, out, row_threads(need, 4), stream);
+  if constexpr (VE == 4) return launch_norm<T, 0, 8>(p, out, row_threads(need, 8), stream);
   return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
 }
 
 // Workgroups whose partial sums of the weight's gradient are kept.
-constexpr size_t kGradParts = 1024;
+constexpr size_t kGradParts = 512;
 
 template <typename T, int TEAM, int NV>
-int launch_grad(const GradParams &p, size_t *parts, hipStream_t stream) {
-  constexpr int THREADS = TEAM < 256 ? 256 : TEAM;
-  constexpr size_t TEAMS = THREADS / TEAM;
+int launch_grad(const GradParams &p, size_t *parts, unsigned threads, hipStream_t stream) {
+  constexpr size_t TEAMS = TEAM ? kWaveTeams : 1;
   size_t grid = (p.rows + TEAMS - 1) / TEAMS;
   if (grid > kGradParts) grid = kGradParts;
   *parts = grid;
-  hipLaunchKernelGGL((rms_norm_grad_kernel<T, TEAM, NV>), dim3((unsigned)grid), dim3(THREADS), 0, stream, p);
+  hipLaunchKernelGGL((rms_norm_grad_kernel<T, TEAM, NV>), dim3((unsigned)grid), dim3(threads), 0, stream, p);
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
@@ -496,13 +498,11 @@ template <typename T> int grad_rows(const GradParams &p, size_t *parts, hipStrea
     return ALAMD_OK;
   }
   const unsigned need = (p.cols + VE - 1) / VE;
-  if (need <= 64) return launch_grad<T, 64, 1>(p, parts, stream);
-  if (need <= 256) return launch_grad<T, 256, 1>(p, parts, stream);
-  if (need <= 512) return launch_grad<T, 256, 2>(p, parts, stream);
-  if (need <= 1024) return launch_grad<T, 256, 4>(p, parts, stream);
-  if (need <= 2048) return launch_grad<T, 1024, 2>(p, parts, stream);
-  if (need <= 4096) return launch_grad<T, 1024, 4>(p, parts, stream);
-  if constexpr (VE == 4) return launch_grad<T, 1024, 8>(p, parts, stream);
+  if (need <= 64) return launch_grad<T, 64, 1>(p, parts, 64 * kWaveTeams, stream);
+  if (need <= 128) return launch_grad<T, 64, 2>(p, parts, 64 * kWaveTeams, stream);
+  if (need <= 2048) return launch_grad<T, 0, 2>(p, parts, row_threads(need, 2), stream);
+  if (need <= 4096) return launch_grad<T, 0, 4>(p, parts, row_threads(need, 4), stream);
+  if constexpr (VE == 4) return launch_grad<T, 0, 8>(p, parts, row_threads(need, 8), stream);
   return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
 }
 
