@@ -5,6 +5,8 @@
 
 namespace alamd {
 
+constexpr int kAuxStoreRow = 2;  // nt
+
 // Element access of a row's type: a 128-bit vector as floats and back (rounded to nearest, ties to even),
 // and single elements.
 template <typename T> struct Row {
@@ -43,112 +45,91 @@ template <typename T> struct Row {
 
 // ---- sums over a team -------------------------------------------------------
 //
-// Butterflies: every lane ends with the same bits, and the order of the additions depends on the team's
-// size alone.  Within 16 lanes the partner comes through a data-parallel move (lanes swapped in pairs,
-// pairs in fours, then mirrored halves of 8 and of 16, whose members already agree), across 16 and 32
-// lanes through the row swaps; the waves of a larger team meet in LDS.
+// A team is a run of whole waves of a workgroup that hold one row together.  Sums and maxima are butterflies:
+// every lane ends with the same bits, and the order of the additions depends on the team's size alone.
+// Within 16 lanes the partner comes through a data-parallel move (lanes swapped in pairs, pairs in fours,
+// then mirrored halves of 8 and of 16, whose members already agree), across 16 and 32 lanes through the row
+// swaps; the waves of a larger team meet in LDS, where the lanes of every wave read one wave's part each.
 
-template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
 }
 constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;
 
-template <int LANES> __device__ __forceinline__ float lanes_sum(float x) {
-  x += __uint_as_float(dpp<kSwap1>(__float_as_uint(x)));
-  x += __uint_as_float(dpp<kSwap2>(__float_as_uint(x)));
-  x += __uint_as_float(dpp<kMirror8>(__float_as_uint(x)));
-  x += __uint_as_float(dpp<kMirror16>(__float_as_uint(x)));
-  if constexpr (LANES > 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  }
-  if constexpr (LANES > 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  }
-  return x;
+// The larger magnitude; a NaN is larger than every number.
+__device__ __forceinline__ float larger(float a, float b) {
+  return __builtin_elementwise_maximum(__builtin_fabsf(a), __builtin_fabsf(b));
 }
-__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
-// The largest of `lanes` neighbouring lanes (a power of two, the same for the whole wave).
-__device__ __forceinline__ uint32_t group_max(uint32_t x, unsigned lanes) {
-  if (lanes > 1) x = umax(x, dpp<kSwap1>(x));
-  if (lanes > 2) x = umax(x, dpp<kSwap2>(x));
-  if (lanes > 4) x = umax(x, dpp<kMirror8>(x));
-  if (lanes > 8) x = umax(x, dpp<kMirror16>(x));
-  if (lanes > 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    x = umax(r[0], r[1]);
-  }
-  if (lanes > 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    x = umax(r[0], r[1]);
+__device__ __forceinline__ float lanes16_sum(float x) {
+  x += dpp<kSwap1>(x);
+  x += dpp<kSwap2>(x);
+  x += dpp<kMirror8>(x);
+  return x + dpp<kMirror16>(x);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x = lanes16_sum(x);
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// The largest magnitude of `lanes` neighbouring lanes: 4, 8, 16, 32 or 64, the same for the whole wave.
+__device__ __forceinline__ float lanes_max(float x, unsigned lanes) {
+  x = larger(x, dpp<kSwap1>(x));
+  x = larger(x, dpp<kSwap2>(x));
+  if (lanes > 4) {
+    x = larger(x, dpp<kMirror8>(x));
+    if (lanes > 8) {
+      x = larger(x, dpp<kMirror16>(x));
+      if (lanes > 16) {
+        auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = larger(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        if (lanes > 32) {
+          r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+          x = larger(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        }
+      }
+    }
   }
   return x;
 }
 
-// The waves of a workgroup of up to 1024 threads meet in `lds`, kWaves * words floats.  A caller that comes back
-// needs another place the next time and may use the first again the time after (a wave that writes there has
-// met all others since).
-constexpr int kWaves = 16;
-template <int TEAM> __device__ __forceinline__ float team_sum(float x, float *lds) {
-  x = lanes_sum<(TEAM ? TEAM : 64)>(x);
-  if constexpr (TEAM == 0) {
-    const unsigned waves = blockDim.x >> 6;
-    if (waves == 1) return x;
-    if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = lds[0];
-    for (unsigned k = 1; k < waves; ++k) x += lds[k];
-  }
-  return x;
-}
-// A sum and a largest word in one meeting.
-template <int TEAM> __device__ __forceinline__ void team_sum_max(float &x, uint32_t &m, float *lds) {
-  x = lanes_sum<(TEAM ? TEAM : 64)>(x);
-  m = group_max(m, TEAM ? TEAM : 64);
-  if constexpr (TEAM == 0) {
-    const unsigned waves = blockDim.x >> 6;
-    if (waves == 1) return;
-    if ((threadIdx.x & 63u) == 0) {
-      lds[2 * (threadIdx.x >> 6)] = x;
-      lds[2 * (threadIdx.x >> 6) + 1] = __uint_as_float(m);
-    }
-    __syncthreads();
-    x = lds[0];
-    m = __float_as_uint(lds[1]);
-    for (unsigned k = 1; k < waves; ++k) {
-      x += lds[2 * k];
-      m = umax(m, __float_as_uint(lds[2 * k + 1]));
-    }
-  }
-}
+constexpr unsigned kMaxWaves = 16;  // of a workgroup
 
 // ---- a row in registers -------------------------------------------------------
 
-// A team is the whole workgroup (TEAM = 0: as many waves as the row needs) or one of its waves (64).  Lane l of
-// a team of n lanes holds the vectors l, n + l, 2 n + l, ..: vector i covers the elements [i * VE, ..) of the row.
-// Where the row does not end with a whole vector, the last one is moved back to end with it: its first `skip`
-// elements are then the lane's before it too.  cols >= VE.
-template <typename T, int TEAM, int NV> struct RowTeam {
-  static_assert(TEAM == 0 || TEAM == 64, "a wave's lanes belong to one row");
+// The workgroup's teams: `teams` of them, `waves` waves each.
+struct TeamShape { unsigned waves, teams; };
+// How rows are read and written (alamd_tile.h says what the policies are): loads past the caches or through
+// them, stores written through or, like the loads past the caches, not kept.
+struct RowPolicy { bool stream_loads, write_through; };
+
+// Lane l of a team of n lanes holds the vectors l, n + l, 2 n + l, ..: vector i covers the elements [i * VE, ..) of
+// the row.  Where the row does not end with a whole vector, the last one is moved back to end with it: its
+// first `skip` elements are then the lane's before it too.  cols >= VE.
+template <typename T, int NV> struct RowTeam {
   static constexpr int VE = Row<T>::VE;
   static constexpr unsigned kNowhere = 0x7ffffff0u;  // an offset behind every row
-  unsigned lane, index, size;
+  unsigned wave, waves, index;  // the wave in the workgroup; waves of the team; which team
+  unsigned lane, size;          // in the team
   unsigned cols;
-  bool ragged;        // the last vector was moved back
+  RowPolicy policy;
+  bool ragged;        // a lane of this wave holds a vector that was moved back
   unsigned off[NV];   // byte offset in the row of the lane's vectors
   unsigned skip[NV];  // elements of each that another lane counts
 
-  __device__ __forceinline__ explicit RowTeam(unsigned n) : cols(n) {
-    size = TEAM ? (unsigned)TEAM : blockDim.x;
-    lane = TEAM ? threadIdx.x % 64u : threadIdx.x;
-    index = TEAM ? (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64u)) : 0u;
+  __device__ __forceinline__ RowTeam(unsigned n, TeamShape shape, RowPolicy how) : cols(n), policy(how) {
+    wave = (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64u));
+    waves = shape.waves;
+    index = shape.teams == 1 ? 0u : wave / waves;
+    size = waves * 64u;
+    lane = threadIdx.x - index * size;
     const unsigned full = n / VE, rem = n % VE;
-    ragged = rem != 0;
+    ragged = rem != 0 && full % size / 64u == wave - index * waves;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const unsigned i = (unsigned)v * size + lane;
-      const bool last = ragged && i == full;
+      const bool last = rem != 0 && i == full;
       off[v] = i < full ? i * 16u : last ? (n - VE) * (unsigned)sizeof(T) : kNowhere;
       skip[v] = last ? VE - rem : 0u;
     }
@@ -158,6 +139,32 @@ template <typename T, int TEAM, int NV> struct RowTeam {
   // Whether element j of vector v is this lane's to count (elements of no row are zeros and may be counted).
   __device__ __forceinline__ bool counts(int v, int j) const { return (unsigned)j >= skip[v]; }
 
+  // The sum over the team.  `lds`: a word for each wave; a caller that comes back needs other words the next
+  // time and may use the first again the time after (a wave that writes there has met all others since).
+  // Every wave of the workgroup has to come.
+  __device__ __forceinline__ float sum(float x, float *lds) const {
+    x = wave_sum(x);
+    if (waves == 1) return x;
+    if ((threadIdx.x & 63u) == 0) lds[wave] = x;
+    __syncthreads();
+    const unsigned k = threadIdx.x & 15u;
+    return lanes16_sum(k < waves ? lds[index * waves + k] : 0.0f);
+  }
+  // A sum and a largest magnitude in one meeting; `lds`: two words for each wave.
+  __device__ __forceinline__ void sum_max(float &x, float &m, float *lds) const {
+    x = wave_sum(x);
+    m = lanes_max(m, 64);
+    if (waves == 1) return;
+    if ((threadIdx.x & 63u) == 0) {
+      lds[wave] = x;
+      lds[kMaxWaves + wave] = m;
+    }
+    __syncthreads();
+    const unsigned k = threadIdx.x & 15u;
+    x = lanes16_sum(k < waves ? lds[index * waves + k] : 0.0f);
+    m = lanes_max(k < waves ? lds[kMaxWaves + index * waves + k] : 0.0f, 16);
+  }
+
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const char *base, unsigned long long pitch, unsigned long long row,
                                                          bool live, unsigned bytes) const {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base + row * pitch), 0, live ? (int)bytes : 0, kRsrcFlags);
@@ -165,21 +172,32 @@ template <typename T, int TEAM, int NV> struct RowTeam {
   __device__ __forceinline__ void load(u32x4 (&raw)[NV], const char *base, unsigned long long pitch, unsigned long long row,
                                        bool live) const {
     const auto r = rsrc(base, pitch, row, live, cols * (unsigned)sizeof(T));
+    if (policy.stream_loads) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) raw[v] = __builtin_amdgcn_raw_buffer_load_b128(r, off[v], 0, kAuxLoadStream);
+      for (int v = 0; v < NV; ++v) raw[v] = __builtin_amdgcn_raw_buffer_load_b128(r, off[v], 0, kAuxLoadStream);
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) raw[v] = __builtin_amdgcn_raw_buffer_load_b128(r, off[v], 0, kAuxLoadCached);
+    }
   }
   __device__ __forceinline__ void store(const u32x4 (&raw)[NV], char *base, unsigned long long pitch, unsigned long long row,
                                         bool live) const {
     const auto r = rsrc(base, pitch, row, live, cols * (unsigned)sizeof(T));
+    if (policy.write_through) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) __builtin_amdgcn_raw_buffer_store_b128(raw[v], r, off[v], 0, kAuxStoreStream);
+      for (int v = 0; v < NV; ++v) __builtin_amdgcn_raw_buffer_store_b128(raw[v], r, off[v], 0, kAuxStoreStream);
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) __builtin_amdgcn_raw_buffer_store_b128(raw[v], r, off[v], 0, kAuxStoreRow);
+    }
   }
+  // A row of weights, of the rows' type or (w32) of fp32; it is read again and again.
   __device__ __forceinline__ void load_weight(float (&w)[VE], int v, const char *weight, int w32) const {
     if constexpr (!std::is_same<T, float>::value) {
       if (w32) {
         const auto r = rsrc(weight, 0, 0, true, cols * 4u);
-        const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(r, off[v] * 2u, 0, 0);
-        const u32x4 b = __builtin_amdgcn_raw_buffer_load_b128(r, off[v] * 2u + 16u, 0, 0);
+        const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(r, off[v] * 2u, 0, kAuxLoadCached);
+        const u32x4 b = __builtin_amdgcn_raw_buffer_load_b128(r, off[v] * 2u + 16u, 0, kAuxLoadCached);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           w[j] = __uint_as_float(a[j]);
@@ -189,11 +207,14 @@ template <typename T, int TEAM, int NV> struct RowTeam {
       }
     }
     const auto r = rsrc(weight, 0, 0, true, cols * (unsigned)sizeof(T));
-    Row<T>::unpack(w, __builtin_amdgcn_raw_buffer_load_b128(r, off[v], 0, 0));
+    Row<T>::unpack(w, __builtin_amdgcn_raw_buffer_load_b128(r, off[v], 0, kAuxLoadCached));
   }
-  // x * by in e4m3, a byte each.  The elements that the lane before has too are left to that lane, whose group's
-  // scale may be another.
-  __device__ __forceinline__ void store_e4m3(const float (&x)[VE], int v, float by, char *base, unsigned long long pitch,
+
+  // x * by in e4m3, a byte each.  `apart`: what a vector that was moved back shares with the lane before belongs
+  // to that lane's group, whose scale is another, and is left to that lane.  (Stores of eight bytes a lane that
+  // split dwords, as in three rows of four of 4099 columns, cost little: 35 us against 32 us at 4104 columns and
+  // 8191 rows.  Whole dwords put together across lanes, with single bytes at both ends of a wave's run, took 51.)
+  __device__ __forceinline__ void store_e4m3(const float (&x)[VE], int v, float by, bool apart, char *base, unsigned long long pitch,
                                              unsigned long long row, bool live) const {
     uint32_t q[VE / 4];
 #pragma unroll
@@ -201,21 +222,39 @@ template <typename T, int TEAM, int NV> struct RowTeam {
       const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * by, x[4 * j + 1] * by, 0, false);
       q[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * by, x[4 * j + 3] * by, lo, true);
     }
-    const unsigned at = off[v] / (unsigned)sizeof(T);
-    const unsigned whole = ragged && skip[v] ? kNowhere : at;
     const auto r = rsrc(base, pitch, row, live, cols);
+    const unsigned at = off[v] / (unsigned)sizeof(T);
+    if (!(apart && ragged)) {
+      store_dwords(q, r, at);
+    } else {
+      store_dwords(q, r, skip[v] ? kNowhere : at);
+      // the rem bytes behind the last whole vector, moved down, in pieces of four, two and one
+      const unsigned rem = cols % VE;
+      unsigned long long tail = VE == 8 ? (unsigned long long)q[VE / 4 - 1] << 32 | q[0] : q[0];
+      tail >>= 8u * (VE - rem);
+      unsigned o = skip[v] ? cols - rem : kNowhere;
+      if (rem & 4u) {
+        __builtin_amdgcn_raw_buffer_store_b32((uint32_t)tail, r, o, 0, 0);
+        tail >>= 32;
+        o += 4u;
+      }
+      if (rem & 2u) {
+        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)tail, r, o, 0, 0);
+        tail >>= 16;
+        o += 2u;
+      }
+      if (rem & 1u) __builtin_amdgcn_raw_buffer_store_b8((uint8_t)tail, r, o, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void store_dwords(const uint32_t (&d)[VE / 4], __amdgpu_buffer_rsrc_t r, unsigned at) const {
     if constexpr (VE == 8) {
       typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-      const u32x2 both = {q[0], q[1]};
-      __builtin_amdgcn_raw_buffer_store_b64(both, r, whole, 0, kAuxStoreStream);
+      const u32x2 both = {d[0], d[1]};
+      if (policy.write_through) __builtin_amdgcn_raw_buffer_store_b64(both, r, at, 0, kAuxStoreStream);
+      else __builtin_amdgcn_raw_buffer_store_b64(both, r, at, 0, kAuxStoreRow);
     } else {
-      __builtin_amdgcn_raw_buffer_store_b32(q[0], r, whole, 0, kAuxStoreStream);
-    }
-    if (ragged && skip[v] && live) {
-      char *o = base + row * pitch + at;
-#pragma unroll
-      for (int j = 1; j < VE; ++j)
-        if (counts(v, j)) o[j] = (char)(q[j / 4] >> (8 * (j % 4)));
+      if (policy.write_through) __builtin_amdgcn_raw_buffer_store_b32(d[0], r, at, 0, kAuxStoreStream);
+      else __builtin_amdgcn_raw_buffer_store_b32(d[0], r, at, 0, kAuxStoreRow);
     }
   }
   // x to elements of an fp32 row.

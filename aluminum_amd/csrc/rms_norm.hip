@@ -37,6 +37,9 @@ struct NormParams {
   int P;
   int w32;          // the weight is fp32 whatever the type of the rows
   unsigned group_log2, groups;  // columns of an 8-bit group, groups of a row
+  int apart;  // a vector that was moved back begins in another 8-bit group than it ends
+  TeamShape shape;
+  RowPolicy policy;
   float eps, inv_n;
 };
 
@@ -45,136 +48,151 @@ enum { OUT_SAME = 0, OUT_E4M3_ROW = 1, OUT_E4M3_GROUP = 2 };
 // The largest value e4m3 holds; the scale of a group whose largest |y| is a is max(a / 448, 2^-126), so that
 // its reciprocal is finite whatever a is.
 constexpr float kE4m3Max = 448.0f, kLeastScale = 1.17549435e-38f;
-__device__ __forceinline__ float scale_of(unsigned amax_bits) {
-  const float a = __uint_as_float(amax_bits) * (1.0f / kE4m3Max);
+__device__ __forceinline__ float scale_of(float amax) {
+  const float a = amax * (1.0f / kE4m3Max);
   return a < kLeastScale ? kLeastScale : a;  // a NaN passes
 }
 
-// Streams whose loads are issued together: eight vectors a lane.
-template <int NV> constexpr int streams_at_once() { return NV >= 8 ? 1 : 8 / NV > 4 ? 4 : 8 / NV; }
+// y / scale = (s * w) * (rstd / scale): the factor for s * w, or, where rstd / scale might not be finite, for y, which
+// then takes the place of s * w.
+template <int VE> __device__ __forceinline__ float quotient_factor(float (&s)[VE], float rstd, float scale) {
+  constexpr float kFar = 1.15292150e18f;  // 2^60
+  const float inv = __builtin_amdgcn_rcpf(scale);
+  if (__ballot(inv > kFar || rstd > kFar) == 0) return rstd * inv;
+#pragma unroll
+  for (int j = 0; j < VE; ++j) s[j] *= rstd;
+  return inv;
+}
 
-// The sum of P streams of a row, in rank order.
-template <int B, typename Team, typename T, int NV, int VE>
-__device__ __forceinline__ void sum_streams(float (&s)[NV][VE], const Team &team, const char *const *in, int P,
+template <typename T, int NV, int VE> __device__ __forceinline__ void add_row(float (&s)[NV][VE], const u32x4 (&raw)[NV]) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    float x[VE];
+    Row<T>::unpack(x, raw[v]);
+#pragma unroll
+    for (int j = 0; j < VE; ++j) s[v][j] += x[j];
+  }
+}
+
+template <typename T, int NV, int VE> __device__ __forceinline__ void set_row(float (&s)[NV][VE], const u32x4 (&raw)[NV]) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v) Row<T>::unpack(s[v], raw[v]);
+}
+
+// Adds streams [from, P) of a row to s, in rank order, the loads of B streams issued together.
+template <int B, typename T, int NV, int VE>
+__device__ __forceinline__ void add_streams(float (&s)[NV][VE], const RowTeam<T, NV> &team, const char *const *in, int from, int P,
                                             unsigned long long pitch, unsigned long long row, bool live) {
-#pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int j = 0; j < VE; ++j) s[v][j] = -0.0f;  // -0 + x is x, whatever x
-  for (int k = 0; k < P; k += B) {
+  for (int k = from; k < P; k += B) {
     u32x4 raw[B][NV];
 #pragma unroll
     for (int b = 0; b < B; ++b)
       if (k + b < P) team.load(raw[b], in[k + b], pitch, row, live);
 #pragma unroll
     for (int b = 0; b < B; ++b)
-      if (k + b < P) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          float x[VE];
-          Row<T>::unpack(x, raw[b][v]);
-#pragma unroll
-          for (int j = 0; j < VE; ++j) s[v][j] += x[j];
-        }
-      }
+      if (k + b < P) add_row<T>(s, raw[b]);
   }
 }
 
-constexpr int kWaveTeams = 4;  // rows, one a wave, of a workgroup whose teams are waves
-
-template <typename T, int TEAM, int NV, int OUT>
-__global__ void __launch_bounds__(TEAM ? 64 * kWaveTeams : 1024) rms_norm_kernel(const NormParams p) {
+// MANY: more than one rank.
+template <typename T, int NV, int OUT, bool MANY>
+__global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
   constexpr int VE = Row<T>::VE;
-  constexpr int TEAMS = TEAM ? kWaveTeams : 1;
-  __shared__ float lds[2][kWaves * 2];
-  const RowTeam<T, TEAM, NV> team(p.cols);
-  int turn = 0;
-  for (unsigned long long r0 = (unsigned long long)blockIdx.x * TEAMS; r0 < p.rows;
-       r0 += (unsigned long long)gridDim.x * TEAMS, turn ^= 1) {
-    const unsigned long long row = r0 + team.index;
-    const bool live = row < p.rows;
-    u32x4 res[NV];
-    if (p.res) team.load(res, p.res, p.res_pitch, row, live);
-    float s[NV][VE];
-    sum_streams<streams_at_once<NV>(), RowTeam<T, TEAM, NV>, T>(s, team, p.in, p.P, p.in_pitch, row, live);
-    if (p.res) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        float x[VE];
-        Row<T>::unpack(x, res[v]);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) s[v][j] += x[j];
-      }
-    }
-    float ss = 0.0f;
-    if (team.ragged) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int j = 0; j < VE; ++j) ss = fmaf(s[v][j], team.counts(v, j) ? s[v][j] : 0.0f, ss);
-    } else {
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int j = 0; j < VE; ++j) ss = fmaf(s[v][j], s[v][j], ss);
-    }
-    u32x4 sum[NV];
-    if (p.sum) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v) sum[v] = Row<T>::pack(s[v]);
-    }
-    if (p.weight) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        float w[VE];
-        team.load_weight(w, v, p.weight, p.w32);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) s[v][j] *= w[j];
-      }
-    }
-    // the largest |s * w| as bits: a NaN is above every number
-    unsigned am = 0;
-    if constexpr (OUT == OUT_E4M3_ROW) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int j = 0; j < VE; ++j) am = umax(am, __float_as_uint(s[v][j]) & 0x7fffffffu);
-      team_sum_max<TEAM>(ss, am, lds[turn]);
-    } else {
-      ss = team_sum<TEAM>(ss, lds[turn]);
-    }
-    // The team has met: every lane has read its part of the row.  Nothing is written before, because a vector
-    // that was moved back reads what another lane writes where the sum takes the residual's place.
-    if (p.sum) team.store(sum, p.sum, p.res_pitch, row, live);
-    const float rstd = rsqrtf(fmaf(ss, p.inv_n, p.eps));
-    if (p.rstd && live && team.lane == 0) p.rstd[row] = rstd;
+  constexpr int B = NV >= 8 ? 1 : NV == 4 ? 2 : 4;
+  __shared__ float lds[kMaxWaves * 2];
+  const RowTeam<T, NV> team(p.cols, p.shape, p.policy);
+  const unsigned long long row = (unsigned long long)blockIdx.x * p.shape.teams + team.index;
+  const bool live = row < p.rows;
+  u32x4 raw[NV];
+  if (p.res) team.load(raw, p.res, p.res_pitch, row, live);
+  float s[NV][VE];
+  if constexpr (MANY) {
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
+      for (int j = 0; j < VE; ++j) s[v][j] = -0.0f;  // -0 + x is x, whatever x
+    add_streams<B>(s, team, p.in, 0, p.P, p.in_pitch, row, live);
+  } else {
+    u32x4 only[NV];
+    team.load(only, p.in[0], p.in_pitch, row, live);
+    set_row<T>(s, only);
+  }
+  if (p.res) add_row<T>(s, raw);
+  float ss = 0.0f;
+  if (team.ragged) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int j = 0; j < VE; ++j) ss = fmaf(s[v][j], team.counts(v, j) ? s[v][j] : 0.0f, ss);
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int j = 0; j < VE; ++j) ss = fmaf(s[v][j], s[v][j], ss);
+  }
+  if (p.sum) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) raw[v] = Row<T>::pack(s[v]);
+  }
+  if (p.weight) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float w[VE];
+      team.load_weight(w, v, p.weight, p.w32);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) s[v][j] *= w[j];
+    }
+  }
+  float am = 0.0f;  // the largest |s * w|
+  if constexpr (OUT == OUT_E4M3_ROW) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int j = 0; j < VE; ++j) am = larger(am, s[v][j]);
+    team.sum_max(ss, am, lds);
+  } else {
+    ss = team.sum(ss, lds);
+  }
+  // The team has met: every lane has read its part of the row.  Nothing is written before, because a vector
+  // that was moved back reads what another lane writes where the sum takes the residual's place.
+  if (p.sum) team.store(raw, p.sum, p.res_pitch, row, live);
+  const float rstd = rsqrtf(fmaf(ss, p.inv_n, p.eps));
+  if (p.rstd && live && team.lane == 0) p.rstd[row] = rstd;
+  if constexpr (OUT == OUT_SAME) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+#pragma unroll
       for (int j = 0; j < VE; ++j) s[v][j] *= rstd;
-    if constexpr (OUT == OUT_SAME) {
+      raw[v] = Row<T>::pack(s[v]);
+    }
+    team.store(raw, p.out, p.out_pitch, row, live);
+  } else if constexpr (OUT == OUT_E4M3_ROW) {
+    const float scale = scale_of(__builtin_fabsf(am * rstd));
+    if (live && team.lane == 0) p.scales[row] = scale;
 #pragma unroll
-      for (int v = 0; v < NV; ++v) sum[v] = Row<T>::pack(s[v]);
-      team.store(sum, p.out, p.out_pitch, row, live);
-    } else {
+    for (int v = 0; v < NV; ++v) {
+      const float by = quotient_factor(s[v], rstd, scale);
+      team.store_e4m3(s[v], v, by, false, p.out, p.out_pitch, row, live);
+    }
+  } else {
+    const unsigned lanes = (1u << p.group_log2) / VE;
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        float scale;
-        if constexpr (OUT == OUT_E4M3_ROW) {
-          scale = scale_of(__float_as_uint(__uint_as_float(am) * rstd) & 0x7fffffffu);
-          if (v == 0 && live && team.lane == 0) p.scales[row] = scale;
-        } else {
-          unsigned a = 0;
+    for (int v = 0; v < NV; ++v) {
+      float a = 0.0f;
+      if (team.ragged) {
 #pragma unroll
-          for (int j = 0; j < VE; ++j) a = umax(a, team.counts(v, j) ? __float_as_uint(s[v][j]) & 0x7fffffffu : 0u);
-          a = group_max(a, (1u << p.group_log2) / VE);
-          scale = scale_of(a);
-          const unsigned e = team.element(v);
-          if (live && e < p.cols && (e & ((1u << p.group_log2) - 1)) == 0)
-            p.scales[row * p.groups + (e >> p.group_log2)] = scale;
-        }
-        team.store_e4m3(s[v], v, __builtin_amdgcn_rcpf(scale), p.out, p.out_pitch, row, live);
+        for (int j = 0; j < VE; ++j) a = larger(a, team.counts(v, j) ? s[v][j] : 0.0f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) a = larger(a, s[v][j]);
       }
+      const float scale = scale_of(__builtin_fabsf(lanes_max(a, lanes) * rstd));
+      // one lane of a group writes its scale; a group behind the row has no place among them
+      const auto r = team.rsrc(reinterpret_cast<const char *>(p.scales), p.groups * 4u, row, live, p.groups * 4u);
+      const unsigned at = (team.lane & (lanes - 1)) == 0 ? (team.element(v) >> p.group_log2) * 4u : team.kNowhere;
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(scale), r, at, 0, 0);
+      const float by = quotient_factor(s[v], rstd, scale);
+      team.store_e4m3(s[v], v, by, p.apart, p.out, p.out_pitch, row, live);
     }
   }
 }
@@ -182,10 +200,9 @@ __global__ void __launch_bounds__(TEAM ? 64 * kWaveTeams : 1024) rms_norm_kernel
 // Rows shorter than a vector: one lane walks a row.
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(256) rms_norm_short_kernel(const NormParams p) {
-  for (unsigned long long row = (unsigned long long)blockIdx.x * 256 + threadIdx.x; row < p.rows;
-       row += (unsigned long long)gridDim.x * 256) {
-    float s[8], ss = 0.0f;
-    unsigned am = 0;
+  const unsigned long long row = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
+  if (row < p.rows) {
+    float s[8], ss = 0.0f, am = 0.0f;
     for (unsigned c = 0; c < p.cols; ++c) {
       float x = 0.0f;
       for (int k = 0; k < p.P; ++k) {
@@ -202,11 +219,10 @@ __global__ void __launch_bounds__(256) rms_norm_short_kernel(const NormParams p)
       if (p.sum) Row<T>::put(p.sum + row * p.res_pitch, c, s[c]);
       const float w = !p.weight ? 1.0f : p.w32 ? Row<float>::get(p.weight, c) : Row<T>::get(p.weight, c);
       s[c] = s[c] * w * rstd;
-      const unsigned b = __float_as_uint(s[c]) & 0x7fffffffu;
-      am = b > am ? b : am;
+      am = larger(am, s[c]);
     }
     if constexpr (E4M3) {
-      const float scale = scale_of(am), by = 1.0f / scale;
+      const float scale = scale_of(am), by = __builtin_amdgcn_rcpf(scale);
       p.scales[row] = scale;
       for (unsigned c = 0; c < p.cols; ++c)
         p.out[row * p.out_pitch + c] = (char)(__builtin_amdgcn_cvt_pk_fp8_f32(s[c] * by, 0.0f, 0, false) & 0xff);
@@ -230,92 +246,147 @@ struct GradParams {
   int P;
   int w32;
   float inv_n;
+  TeamShape shape;
+  RowPolicy policy;
 };
 
-template <typename T, int TEAM, int NV>
-__global__ void __launch_bounds__(TEAM ? 64 * kWaveTeams : 1024) rms_norm_grad_kernel(const GradParams p) {
+// What is read of a row up front: x, dsum, rstd and B of the ranks' gradients.
+template <typename T, int NV, int B> struct Fetched {
+  u32x4 x[NV], ds[NV], dy[B][NV];
+  float rstd;
+  __device__ __forceinline__ void fetch(const GradParams &p, const RowTeam<T, NV> &team, unsigned long long row) {
+    const bool live = row < p.rows;
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (b < p.P) team.load(dy[b], p.dy[b], p.dy_pitch, row, live);
+    team.load(x, p.x, p.x_pitch, row, live);
+    if (p.dsum) team.load(ds, p.dsum, p.dsum_pitch, row, live);
+    rstd = live ? p.rstd[row] : 0.0f;
+  }
+};
+
+// WIDE: rows of so many vectors a lane that the weight's gradient is kept in LDS and nothing is read ahead.
+template <typename T, int NV, int B, bool WIDE, int THREADS>
+__global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams p) {
   constexpr int VE = Row<T>::VE;
-  constexpr int TEAMS = TEAM ? kWaveTeams : 1;
-  __shared__ float lds[2][kWaves];
-  const RowTeam<T, TEAM, NV> team(p.cols);
-  float dw[NV][VE];
+  __shared__ float lds[2][kMaxWaves];
+  extern __shared__ float4 kept[];  // WIDE: the weight's gradient; else room for one team to hand it to the next
+  const RowTeam<T, NV> team(p.cols, p.shape, p.policy);
+  auto slot = [&](int v, int j) -> float4 & { return kept[(unsigned)(v * (VE / 4) + j / 4) * team.size + team.lane]; };
+  float dw[WIDE ? 1 : NV][VE], w[WIDE ? 1 : NV][VE];
+  if constexpr (WIDE) {
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v)
 #pragma unroll
-    for (int j = 0; j < VE; ++j) dw[v][j] = 0.0f;
+      for (int j = 0; j < VE; j += 4) slot(v, j) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        dw[v][j] = 0.0f;
+        w[v][j] = 1.0f;
+      }
+      if (p.weight) team.load_weight(w[v], v, p.weight, p.w32);
+    }
+  }
   int turn = 0;
-  for (unsigned long long r0 = (unsigned long long)blockIdx.x * TEAMS; r0 < p.rows;
-       r0 += (unsigned long long)gridDim.x * TEAMS, turn ^= 1) {
+  const unsigned long long step = (unsigned long long)gridDim.x * p.shape.teams;
+  unsigned long long r0 = (unsigned long long)blockIdx.x * p.shape.teams;
+  Fetched<T, NV, B> next;
+  if constexpr (!WIDE) next.fetch(p, team, r0 + team.index);
+  for (; r0 < p.rows; r0 += step, turn ^= 1) {
     const unsigned long long row = r0 + team.index;
     const bool live = row < p.rows;
-    u32x4 xr[NV], ds[NV];
-    team.load(xr, p.x, p.x_pitch, row, live);
-    if (p.dsum) team.load(ds, p.dsum, p.dsum_pitch, row, live);
-    const float rstd = live ? p.rstd[row] : 0.0f;
+    if constexpr (WIDE) next.fetch(p, team, row);
+    Fetched<T, NV, B> now = next;
+    // the next row's loads are on their way while this one's sum is made and its gradient written
+    if constexpr (!WIDE) next.fetch(p, team, row + step);
     float g[NV][VE];
-    sum_streams<streams_at_once<NV>(), RowTeam<T, TEAM, NV>, T>(g, team, p.dy, p.P, p.dy_pitch, row, live);
+    set_row<T>(g, now.dy[0]);
+#pragma unroll
+    for (int b = 1; b < B; ++b)
+      if (b < p.P) add_row<T>(g, now.dy[b]);
+    add_streams<(NV >= 8 ? 1 : NV == 4 ? 2 : 4)>(g, team, p.dy, B, p.P, p.dy_pitch, row, live);
     float dot = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float x[VE], w[VE];
-      Row<T>::unpack(x, xr[v]);
-      if (p.weight) team.load_weight(w, v, p.weight, p.w32);
+      if constexpr (NV >= 4) __builtin_amdgcn_sched_barrier(0);  // one vector after another: registers are short
+      float x[VE], wv[VE], d[VE];
+      Row<T>::unpack(x, now.x[v]);
+      if constexpr (WIDE) {
 #pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        const float n = x[j] * rstd;
-        // a row that is not there has rstd = 0 and reads zeros
-        dw[v][j] = fmaf(g[v][j], n, dw[v][j]);
-        if (p.weight) g[v][j] *= w[j];
-        dot = fmaf(g[v][j], team.counts(v, j) ? n : 0.0f, dot);
-      }
-    }
-    if (p.dx) {
-      const float c = team_sum<TEAM>(dot, lds[turn]) * p.inv_n;
+        for (int j = 0; j < VE; ++j) wv[j] = 1.0f;
+        if (p.weight) team.load_weight(wv, v, p.weight, p.w32);
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        float x[VE];
-        Row<T>::unpack(x, xr[v]);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) g[v][j] = rstd * fmaf(-(x[j] * rstd), c, g[v][j]);
-      }
-      // (dsum was read before the team met: dx may take its place)
-      if (p.dsum) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          float d[VE];
-          Row<T>::unpack(d, ds[v]);
-#pragma unroll
-          for (int j = 0; j < VE; ++j) g[v][j] += d[j];
+        for (int j = 0; j < VE; j += 4) {
+          const float4 a = slot(v, j);
+          d[j] = a.x, d[j + 1] = a.y, d[j + 2] = a.z, d[j + 3] = a.w;
         }
       }
 #pragma unroll
-      for (int v = 0; v < NV; ++v) ds[v] = Row<T>::pack(g[v]);
-      team.store(ds, p.dx, p.dx_pitch, row, live);
+      for (int j = 0; j < VE; ++j) {
+        const float n = x[j] * now.rstd;
+        // a row that is not there has rstd = 0 and reads zeros
+        if constexpr (WIDE) d[j] = fmaf(g[v][j], n, d[j]);
+        else dw[v][j] = fmaf(g[v][j], n, dw[v][j]);
+        g[v][j] *= WIDE ? wv[j] : w[WIDE ? 0 : v][j];
+        dot = fmaf(g[v][j], !team.ragged || team.counts(v, j) ? n : 0.0f, dot);
+      }
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int j = 0; j < VE; j += 4) slot(v, j) = make_float4(d[j], d[j + 1], d[j + 2], d[j + 3]);
+      }
+    }
+    if (p.dx) {
+      const float c = team.sum(dot, lds[turn]) * p.inv_n;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        if constexpr (NV >= 4) __builtin_amdgcn_sched_barrier(0);
+        float x[VE];
+        asm volatile("" : "+v"(now.x[v]));  // x is widened again, not kept as floats
+        Row<T>::unpack(x, now.x[v]);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) g[v][j] = now.rstd * fmaf(-(x[j] * now.rstd), c, g[v][j]);
+      }
+      // (dsum was read before the team met: dx may take its place)
+      if (p.dsum) add_row<T>(g, now.ds);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) now.x[v] = Row<T>::pack(g[v]);
+      team.store(now.x, p.dx, p.dx_pitch, row, live);
     }
   }
   if (!p.partial) return;
   float *dst = p.partial + (size_t)blockIdx.x * p.cols;
-  if constexpr (TEAMS == 1) {
+  if constexpr (WIDE) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) team.store_f32(dw[v], v, dst);
+    for (int v = 0; v < NV; ++v) {
+      float d[VE];
+#pragma unroll
+      for (int j = 0; j < VE; j += 4) {
+        const float4 a = slot(v, j);
+        d[j] = a.x, d[j + 1] = a.y, d[j + 2] = a.z, d[j + 3] = a.w;
+      }
+      team.store_f32(d, v, dst);
+    }
   } else {
     // the teams of the workgroup one after another, in their order
-    __shared__ float part[TEAM * NV * VE];
-    for (int t = 0; t < TEAMS; ++t) {
-      if ((int)team.index == t) {
+    for (unsigned t = 0; t < p.shape.teams; ++t) {
+      if (t > 0) __syncthreads();
+      if (team.index != t) continue;
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+      for (int v = 0; v < NV; ++v) {
 #pragma unroll
-          for (int j = 0; j < VE; ++j) {
-            float &a = part[(v * VE + j) * TEAM + team.lane];
-            dw[v][j] = t == 0 ? dw[v][j] : a + dw[v][j];
-            a = dw[v][j];
+        for (int j = 0; j < VE; j += 4) {
+          if (t > 0) {
+            const float4 a = slot(v, j);
+            dw[v][j] = a.x + dw[v][j], dw[v][j + 1] = a.y + dw[v][j + 1], dw[v][j + 2] = a.z + dw[v][j + 2],
+            dw[v][j + 3] = a.w + dw[v][j + 3];
           }
-        if (t == TEAMS - 1)
-#pragma unroll
-          for (int v = 0; v < NV; ++v) team.store_f32(dw[v], v, dst);
+          if (t + 1 < p.shape.teams) slot(v, j) = make_float4(dw[v][j], dw[v][j + 1], dw[v][j + 2], dw[v][j + 3]);
+        }
+        if (t + 1 == p.shape.teams) team.store_f32(dw[v], v, dst);
       }
-      __syncthreads();
     }
   }
 }
@@ -365,13 +436,18 @@ __global__ void __launch_bounds__(1024) rms_norm_dweight_kernel(char *dw, const 
   const unsigned c = threadIdx.x & 31u, slice = threadIdx.x >> 5, col = blockIdx.x * 32u + c;
   float a = 0.0f;
   if (col < cols) {
-    const unsigned per = (parts + 31u) / 32u;
-    const unsigned from = slice * per, to = from + per < parts ? from + per : parts;
-    for (unsigned k = from; k < to; ++k) a += partial[(size_t)k * cols + col];
+    for (unsigned k = slice; k < parts; k += 32u * 8u) {
+      float x[8];
+#pragma unroll
+      for (unsigned u = 0; u < 8; ++u) x[u] = k + u * 32u < parts ? partial[(size_t)(k + u * 32u) * cols + col] : 0.0f;
+#pragma unroll
+      for (unsigned u = 0; u < 8; ++u) a += x[u];
+    }
   }
   lds[slice][c] = a;
   __syncthreads();
   if (slice == 0 && col < cols) {
+#pragma unroll
     for (int k = 1; k < 32; ++k) a += lds[k][c];
     Row<W>::put(dw, col, a);
   }
@@ -436,58 +512,82 @@ int check_common(int P, size_t cols, int dtype, const void *weight, int weight_d
   return ALAMD_OK;
 }
 
-// Rows a launch has workgroups for; a workgroup that has done its row takes the next one that far on.
+// Workgroups of a launch; what is left is done by further ones.
 constexpr size_t kMaxGrid = (size_t)1 << 21;
 
-template <typename T, int TEAM, int NV>
-int launch_norm(const NormParams &p, int out, unsigned threads, hipStream_t stream) {
-  constexpr size_t TEAMS = TEAM ? kWaveTeams : 1;
-  size_t grid = (p.rows + TEAMS - 1) / TEAMS;
-  if (grid > kMaxGrid) grid = kMaxGrid;
-  auto kern = out == OUT_SAME ? rms_norm_kernel<T, TEAM, NV, OUT_SAME>
-              : out == OUT_E4M3_ROW ? rms_norm_kernel<T, TEAM, NV, OUT_E4M3_ROW> : rms_norm_kernel<T, TEAM, NV, OUT_E4M3_GROUP>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(threads), 0, stream, p);
+// A call that moves less than this reads through the caches.
+constexpr size_t kStreamFromBytes = (size_t)256 << 20;
+
+inline unsigned waves_for(unsigned need, unsigned nv) { return (need + 64 * nv - 1) / (64 * nv); }
+
+// The call on the rows from the first `done` on.
+inline NormParams from_row(NormParams p, size_t done) {
+  for (int k = 0; k < p.P; ++k) p.in[k] += done * p.in_pitch;
+  if (p.res) p.res += done * p.res_pitch;
+  if (p.sum) p.sum += done * p.res_pitch;
+  p.out += done * p.out_pitch;
+  if (p.rstd) p.rstd += done;
+  if (p.scales) p.scales += done * p.groups;
+  p.rows -= done;
+  return p;
+}
+
+// Launches `kern`, whose workgroups have `threads` threads and do `per` rows each.
+inline int launch_rows(void (*kern)(NormParams), const NormParams &p, size_t per, unsigned threads, hipStream_t stream) {
+  for (size_t done = 0; done < p.rows; done += kMaxGrid * per) {
+    const size_t left = (p.rows - done + per - 1) / per;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(left < kMaxGrid ? left : kMaxGrid)), dim3(threads), 0, stream,
+                       done ? from_row(p, done) : p);
+  }
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
 
-// Threads of a workgroup that holds a row of `need` vectors, nv of them a lane.
-inline unsigned row_threads(unsigned need, unsigned nv) { return ((need + nv - 1) / nv + 63u) & ~63u; }
+template <typename T, int NV> int launch_norm(NormParams &p, int out, unsigned waves, unsigned teams, hipStream_t stream) {
+  p.shape = {waves, teams};
+  auto kern = out == OUT_SAME ? (p.P > 1 ? rms_norm_kernel<T, NV, OUT_SAME, true> : rms_norm_kernel<T, NV, OUT_SAME, false>)
+              : out == OUT_E4M3_ROW ? (p.P > 1 ? rms_norm_kernel<T, NV, OUT_E4M3_ROW, true> : rms_norm_kernel<T, NV, OUT_E4M3_ROW, false>)
+              : (p.P > 1 ? rms_norm_kernel<T, NV, OUT_E4M3_GROUP, true> : rms_norm_kernel<T, NV, OUT_E4M3_GROUP, false>);
+  return launch_rows(kern, p, teams, 64 * waves * teams, stream);
+}
 
-template <typename T> int norm_rows(const NormParams &p, int out, hipStream_t stream) {
+template <typename T> int norm_rows(NormParams &p, int out, hipStream_t stream) {
   constexpr unsigned VE = Row<T>::VE;
-  if (p.cols < VE) {
-    size_t grid = (p.rows + 255) / 256;
-    if (grid > kMaxGrid) grid = kMaxGrid;
-    hipLaunchKernelGGL(out == OUT_SAME ? (rms_norm_short_kernel<T, false>) : (rms_norm_short_kernel<T, true>), dim3((unsigned)grid),
-                       dim3(256), 0, stream, p);
-    ALAMD_HIP(hipGetLastError());
-    return ALAMD_OK;
-  }
+  if (p.cols < VE)
+    return launch_rows(out == OUT_SAME ? rms_norm_short_kernel<T, false> : rms_norm_short_kernel<T, true>, p, 256, 256, stream);
   const unsigned need = (p.cols + VE - 1) / VE;  // vectors of a row
-  if (need <= 64) return launch_norm<T, 64, 1>(p, out, 64 * kWaveTeams, stream);
-  if (need <= 128) return launch_norm<T, 64, 2>(p, out, 64 * kWaveTeams, stream);
-  if (need <= 2048) return launch_norm<T, 0, 2>(p, out, row_threads(need, 2), stream);
-  if (need <= 4096) return launch_norm<T, 0, 4>(p, out, row_threads(need, 4), stream);
-  if constexpr (VE == 4) return launch_norm<T, 0, 8>(p, out, row_threads(need, 8), stream);
+  if (need <= 64) return launch_norm<T, 1>(p, out, 1, 4, stream);
+  if (p.rows <= 512 && need <= 1024) return launch_norm<T, 1>(p, out, waves_for(need, 1), 1, stream);
+  if (need <= 128) return launch_norm<T, 2>(p, out, 1, 4, stream);
+  if (need <= 2048) return launch_norm<T, 2>(p, out, waves_for(need, 2), 1, stream);
+  if (need <= 4096) return launch_norm<T, 4>(p, out, waves_for(need, 4), 1, stream);
+  if constexpr (VE == 4) return launch_norm<T, 8>(p, out, waves_for(need, 8), 1, stream);
   return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
 }
 
 // Workgroups whose partial sums of the weight's gradient are kept.
-constexpr size_t kGradParts = 512;
+constexpr size_t kGradParts = 256;
 
-template <typename T, int TEAM, int NV>
-int launch_grad(const GradParams &p, size_t *parts, unsigned threads, hipStream_t stream) {
-  constexpr size_t TEAMS = TEAM ? kWaveTeams : 1;
-  size_t grid = (p.rows + TEAMS - 1) / TEAMS;
+template <typename T, int NV, int B, bool WIDE, int THREADS = 512>
+int launch_grad_b(GradParams &p, size_t *parts, unsigned waves, unsigned teams, hipStream_t stream) {
+  p.shape = {waves, teams};
+  size_t grid = (p.rows + teams - 1) / teams;
   if (grid > kGradParts) grid = kGradParts;
   *parts = grid;
-  hipLaunchKernelGGL((rms_norm_grad_kernel<T, TEAM, NV>), dim3((unsigned)grid), dim3(threads), 0, stream, p);
+  const size_t lds = WIDE || teams > 1 ? (size_t)waves * 64 * NV * Row<T>::VE * sizeof(float) : 0;
+  hipLaunchKernelGGL((rms_norm_grad_kernel<T, NV, B, WIDE, THREADS>), dim3((unsigned)grid), dim3(64 * waves * teams), lds, stream, p);
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
+template <typename T, int NV> int launch_grad(GradParams &p, size_t *parts, unsigned waves, hipStream_t stream) {
+  unsigned teams = 8 / waves;
+  while (teams > 1 && p.rows < (size_t)256 * teams) teams /= 2;
+  if (teams < 1) teams = 1;
+  return p.P == 1 ? launch_grad_b<T, NV, 1, false>(p, parts, waves, teams, stream)
+                  : launch_grad_b<T, NV, 4, false>(p, parts, waves, teams, stream);
+}
 
-template <typename T> int grad_rows(const GradParams &p, size_t *parts, hipStream_t stream) {
+template <typename T> int grad_rows(GradParams &p, size_t *parts, hipStream_t stream) {
   constexpr unsigned VE = Row<T>::VE;
   if (p.cols < VE) {
     size_t grid = (p.rows + 255) / 256;
@@ -498,11 +598,11 @@ template <typename T> int grad_rows(const GradParams &p, size_t *parts, hipStrea
     return ALAMD_OK;
   }
   const unsigned need = (p.cols + VE - 1) / VE;
-  if (need <= 64) return launch_grad<T, 64, 1>(p, parts, 64 * kWaveTeams, stream);
-  if (need <= 128) return launch_grad<T, 64, 2>(p, parts, 64 * kWaveTeams, stream);
-  if (need <= 2048) return launch_grad<T, 0, 2>(p, parts, row_threads(need, 2), stream);
-  if (need <= 4096) return launch_grad<T, 0, 4>(p, parts, row_threads(need, 4), stream);
-  if constexpr (VE == 4) return launch_grad<T, 0, 8>(p, parts, row_threads(need, 8), stream);
+  if (need <= 64) return launch_grad<T, 1>(p, parts, 1, stream);
+  if (need <= 1024) return launch_grad<T, 2>(p, parts, waves_for(need, 2), stream);
+  if (need <= 2048) return launch_grad_b<T, 4, 1, false>(p, parts, waves_for(need, 4), 1, stream);
+  if (need <= 4096) return launch_grad_b<T, 8, 1, true>(p, parts, waves_for(need, 8), 1, stream);
+  if constexpr (VE == 4) return launch_grad_b<T, 8, 1, true, 1024>(p, parts, waves_for(need, 8), 1, stream);
   return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
 }
 
@@ -563,6 +663,11 @@ int alamd_rms_norm(void *out, size_t out_stride, void *sum, const void *residual
   p.groups = (unsigned)groups;
   p.eps = eps;
   p.inv_n = 1.0f / (float)cols;
+  p.apart = cols % (16 / es) != 0 && (cols - cols % (16 / es)) % (group ? group : cols) == 0;
+  const size_t moved = rows * cols * (es * ((size_t)P + (residual ? 1 : 0) + (sum ? 1 : 0)) + oes);
+  const auto lines = [](const void *at, size_t pitch) { return ((reinterpret_cast<uintptr_t>(at) | pitch) & 63u) == 0; };
+  p.policy = {moved >= kStreamFromBytes,
+              moved >= kStreamFromBytes && lines(out, p.out_pitch) && (!sum || lines(sum, p.res_pitch))};
   const int kind = !scales ? OUT_SAME : group == 0 || group >= cols ? OUT_E4M3_ROW : OUT_E4M3_GROUP;
   switch (dtype) {
   case ALAMD_F16: return norm_rows<f16_t>(p, kind, as_stream(stream));
@@ -629,6 +734,9 @@ int alamd_rms_norm_grad(void *dx, size_t dx_stride, const void *const *dys, int 
     p.P = P;
     p.w32 = weight && weight_dtype == ALAMD_F32;
     p.inv_n = 1.0f / (float)cols;
+    const size_t moved = rows * cols * es * ((size_t)P + 1 + (dsum ? 1 : 0) + (dx ? 1 : 0));
+    p.policy = {moved >= kStreamFromBytes,
+                moved >= kStreamFromBytes && ((reinterpret_cast<uintptr_t>(dx) | p.dx_pitch) & 63u) == 0};
     switch (dtype) {
     case ALAMD_F16: rc = grad_rows<f16_t>(p, &parts, as_stream(stream)); break;
     case ALAMD_BF16: rc = grad_rows<bf16_t>(p, &parts, as_stream(stream)); break;
