@@ -269,8 +269,9 @@ template <typename T, int NV, int B> struct Fetched {
 template <typename T, int NV, int B, bool WIDE, int THREADS>
 __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams p) {
   constexpr int VE = Row<T>::VE;
+  constexpr bool AHEAD = !(WIDE || (NV == 2 && THREADS > 512));  // the next row is read ahead
   __shared__ float lds[2][kMaxWaves];
-  extern __shared__ float4 kept[];  // WIDE: the weight's gradient; else room for one team to hand it to the next
+  extern __shared__ float4 kept[];  // WIDE: the weight's gradient; else room for half of the teams to hand it over
   const RowTeam<T, NV> team(p.cols, p.shape, p.policy);
   auto slot = [&](int v, int j) -> float4 & { return kept[(unsigned)(v * (VE / 4) + j / 4) * team.size + team.lane]; };
   float dw[WIDE ? 1 : NV][VE], w[WIDE ? 1 : NV][VE];
@@ -294,20 +295,20 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
   const unsigned long long step = (unsigned long long)gridDim.x * p.shape.teams;
   unsigned long long r0 = (unsigned long long)blockIdx.x * p.shape.teams;
   Fetched<T, NV, B> next;
-  if constexpr (!WIDE) next.fetch(p, team, r0 + team.index);
+  if constexpr (AHEAD) next.fetch(p, team, r0 + team.index);
   for (; r0 < p.rows; r0 += step, turn ^= 1) {
     const unsigned long long row = r0 + team.index;
     const bool live = row < p.rows;
-    if constexpr (WIDE) next.fetch(p, team, row);
+    if constexpr (!AHEAD) next.fetch(p, team, row);
     Fetched<T, NV, B> now = next;
     // the next row's loads are on their way while this one's sum is made and its gradient written
-    if constexpr (!WIDE) next.fetch(p, team, row + step);
+    if constexpr (AHEAD) next.fetch(p, team, row + step);
     float g[NV][VE];
     set_row<T>(g, now.dy[0]);
 #pragma unroll
     for (int b = 1; b < B; ++b)
       if (b < p.P) add_row<T>(g, now.dy[b]);
-    add_streams<(NV >= 8 ? 1 : NV == 4 ? 2 : 4)>(g, team, p.dy, B, p.P, p.dy_pitch, row, live);
+    add_streams<(WIDE ? 1 : 4)>(g, team, p.dy, B, p.P, p.dy_pitch, row, live);
     float dot = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -370,23 +371,35 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
       team.store_f32(d, v, dst);
     }
   } else {
-    // the teams of the workgroup one after another, in their order
-    for (unsigned t = 0; t < p.shape.teams; ++t) {
-      if (t > 0) __syncthreads();
-      if (team.index != t) continue;
+    // the upper half of the teams hands its part to the lower half, until one team has all
+    for (unsigned n = p.shape.teams; n > 1;) {
+      const unsigned half = (n + 1) / 2;
+      const unsigned room = NV * (VE / 4) * team.size;
+      if (team.index >= half && team.index < n) {
+        float4 *to = kept + (team.index - half) * room;
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int j = 0; j < VE; j += 4) {
-          if (t > 0) {
-            const float4 a = slot(v, j);
-            dw[v][j] = a.x + dw[v][j], dw[v][j + 1] = a.y + dw[v][j + 1], dw[v][j + 2] = a.z + dw[v][j + 2],
-            dw[v][j + 3] = a.w + dw[v][j + 3];
-          }
-          if (t + 1 < p.shape.teams) slot(v, j) = make_float4(dw[v][j], dw[v][j + 1], dw[v][j + 2], dw[v][j + 3]);
-        }
-        if (t + 1 == p.shape.teams) team.store_f32(dw[v], v, dst);
+          for (int j = 0; j < VE; j += 4)
+            to[(unsigned)(v * (VE / 4) + j / 4) * team.size + team.lane] = make_float4(dw[v][j], dw[v][j + 1], dw[v][j + 2], dw[v][j + 3]);
       }
+      __syncthreads();
+      if (team.index < n - half) {
+        const float4 *from = kept + team.index * room;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int j = 0; j < VE; j += 4) {
+            const float4 a = from[(unsigned)(v * (VE / 4) + j / 4) * team.size + team.lane];
+            dw[v][j] += a.x, dw[v][j + 1] += a.y, dw[v][j + 2] += a.z, dw[v][j + 3] += a.w;
+          }
+      }
+      __syncthreads();
+      n = half;
+    }
+    if (team.index == 0) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) team.store_f32(dw[v], v, dst);
     }
   }
 }
@@ -568,23 +581,22 @@ template <typename T> int norm_rows(NormParams &p, int out, hipStream_t stream) 
 // Workgroups whose partial sums of the weight's gradient are kept.
 constexpr size_t kGradParts = 256;
 
-template <typename T, int NV, int B, bool WIDE, int THREADS = 512>
+template <typename T, int NV, int B, bool WIDE, int THREADS>
 int launch_grad_b(GradParams &p, size_t *parts, unsigned waves, unsigned teams, hipStream_t stream) {
   p.shape = {waves, teams};
   size_t grid = (p.rows + teams - 1) / teams;
   if (grid > kGradParts) grid = kGradParts;
   *parts = grid;
-  const size_t lds = WIDE || teams > 1 ? (size_t)waves * 64 * NV * Row<T>::VE * sizeof(float) : 0;
+  const size_t lds = (WIDE ? 1 : teams / 2) * (size_t)waves * 64 * NV * Row<T>::VE * sizeof(float);
   hipLaunchKernelGGL((rms_norm_grad_kernel<T, NV, B, WIDE, THREADS>), dim3((unsigned)grid), dim3(64 * waves * teams), lds, stream, p);
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
-template <typename T, int NV> int launch_grad(GradParams &p, size_t *parts, unsigned waves, hipStream_t stream) {
-  unsigned teams = 8 / waves;
-  while (teams > 1 && p.rows < (size_t)256 * teams) teams /= 2;
-  if (teams < 1) teams = 1;
-  return p.P == 1 ? launch_grad_b<T, NV, 1, false>(p, parts, waves, teams, stream)
-                  : launch_grad_b<T, NV, 4, false>(p, parts, waves, teams, stream);
+template <typename T, int NV, int THREADS> int launch_grad(GradParams &p, size_t *parts, unsigned waves, hipStream_t stream) {
+  unsigned teams = THREADS / 64 / waves;
+  while (teams > 1 && p.rows < (size_t)256 * teams) --teams;
+  return p.P == 1 ? launch_grad_b<T, NV, 1, false, THREADS>(p, parts, waves, teams, stream)
+                  : launch_grad_b<T, NV, 4, false, THREADS>(p, parts, waves, teams, stream);
 }
 
 template <typename T> int grad_rows(GradParams &p, size_t *parts, hipStream_t stream) {
@@ -598,10 +610,10 @@ template <typename T> int grad_rows(GradParams &p, size_t *parts, hipStream_t st
     return ALAMD_OK;
   }
   const unsigned need = (p.cols + VE - 1) / VE;
-  if (need <= 64) return launch_grad<T, 1>(p, parts, 1, stream);
-  if (need <= 1024) return launch_grad<T, 2>(p, parts, waves_for(need, 2), stream);
-  if (need <= 2048) return launch_grad_b<T, 4, 1, false>(p, parts, waves_for(need, 4), 1, stream);
-  if (need <= 4096) return launch_grad_b<T, 8, 1, true>(p, parts, waves_for(need, 8), 1, stream);
+  if (need <= 640) return launch_grad<T, 1, 1024>(p, parts, waves_for(need, 1), stream);
+  if (need <= 1024) return launch_grad<T, 2, 512>(p, parts, waves_for(need, 2), stream);
+  if (need <= 2048) return launch_grad_b<T, 2, 1, false, 1024>(p, parts, waves_for(need, 2), 1, stream);
+  if (need <= 4096) return launch_grad_b<T, 4, 1, true, 1024>(p, parts, waves_for(need, 4), 1, stream);
   if constexpr (VE == 4) return launch_grad_b<T, 8, 1, true, 1024>(p, parts, waves_for(need, 8), 1, stream);
   return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
 }
