@@ -54,7 +54,7 @@ template <typename T> struct Row {
 template <int CTRL> __device__ __forceinline__ float dpp(float x) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
 }
-constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;
+constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140, kFromLaneBehind = 0x130;
 
 // The larger magnitude; a NaN is larger than every number.
 __device__ __forceinline__ float larger(float a, float b) {
@@ -104,10 +104,20 @@ struct TeamShape { unsigned waves, teams; };
 // them, stores written through or, like the loads past the caches, not kept.
 struct RowPolicy { bool stream_loads, write_through; };
 
-// Lane l of a team of n lanes holds the vectors l, n + l, 2 n + l, ..: vector i covers the elements [i * VE, ..) of
-// the row.  Where the row does not end with a whole vector, the last one is moved back to end with it: its
-// first `skip` elements are then the lane's before it too.  cols >= VE.
-template <typename T, int NV> struct RowTeam {
+// Vector i of a row covers its elements [i * VE, ..); every wave of a team holds NV runs of 64 vectors, one a
+// lane, and the waves' runs follow one another.  Where the row does not end with a whole vector, the last one
+// is moved back to end with it: its first `skip` elements are then the lane's before it too.  cols >= VE.
+//
+// HALVES: rows of 16-bit elements may start in the middle of a dword, as every other row of an odd number of
+// columns does, and every load of such a row would split dwords (forward pass over 16384 rows of 5125 bf16 to
+// rows of an even pitch: one stream 73 us, two 117 us; from rows of an even pitch 63 and 84).  It is read from
+// the dword it starts in instead - the two bytes before it that come along share that dword -, and `settle`
+// moves every lane's elements down by one, the last coming from the next lane, or, at the end of a wave's run,
+// from a dword that the wave reads as a scalar: 65 and 93 us.  The backward pass lets loads split dwords: it is
+// bound by its instructions there, and what the moves cost (12 a vector and stream) is what the loads gain (121 us
+// either way); with the next row's scalars under way, every meeting of a team would wait for them besides (207 us).
+template <typename T, int NV, bool HALVES> struct RowTeam {
+  static_assert(!HALVES || sizeof(T) == 2, "only 16-bit elements start in the middle of a dword");
   static constexpr int VE = Row<T>::VE;
   static constexpr unsigned kNowhere = 0x7ffffff0u;  // an offset behind every row
   unsigned wave, waves, index;  // the wave in the workgroup; waves of the team; which team
@@ -128,14 +138,14 @@ template <typename T, int NV> struct RowTeam {
     ragged = rem != 0 && full % size / 64u == wave - index * waves;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const unsigned i = (unsigned)v * size + lane;
+      const unsigned i = vector(v);
       const bool last = rem != 0 && i == full;
       off[v] = i < full ? i * 16u : last ? (n - VE) * (unsigned)sizeof(T) : kNowhere;
       skip[v] = last ? VE - rem : 0u;
     }
   }
-  // The first element of vector v, counted as if every vector were in its place.
-  __device__ __forceinline__ unsigned element(int v) const { return ((unsigned)v * size + lane) * VE; }
+  // The vector that the lane holds as its v-th, counted as if every one were in its place.
+  __device__ __forceinline__ unsigned vector(int v) const { return (unsigned)v * size + lane; }
   // Whether element j of vector v is this lane's to count (elements of no row are zeros and may be counted).
   __device__ __forceinline__ bool counts(int v, int j) const { return (unsigned)j >= skip[v]; }
 
@@ -169,15 +179,60 @@ template <typename T, int NV> struct RowTeam {
                                                          bool live, unsigned bytes) const {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base + row * pitch), 0, live ? (int)bytes : 0, kRsrcFlags);
   }
-  __device__ __forceinline__ void load(u32x4 (&raw)[NV], const char *base, unsigned long long pitch, unsigned long long row,
+  // A lane's part of a row as it is in memory, and the dwords behind the wave's runs.
+  struct Loaded {
+    u32x4 raw[NV];
+    uint32_t more[HALVES ? NV : 1];
+  };
+  static __device__ __forceinline__ bool split(const char *base, unsigned long long pitch, unsigned long long row) {
+    return HALVES && ((reinterpret_cast<uintptr_t>(base) + row * pitch) & 2u) != 0;
+  }
+  __device__ __forceinline__ void load(Loaded &to, const char *base, unsigned long long pitch, unsigned long long row,
                                        bool live) const {
-    const auto r = rsrc(base, pitch, row, live, cols * (unsigned)sizeof(T));
+    const unsigned back = split(base, pitch, row) ? 2u : 0u;
+    const auto r = rsrc(base - back, pitch, row, live, cols * (unsigned)sizeof(T) + back);
+    unsigned at[NV];  // (the vector that was moved back is read from where it begins)
+#pragma unroll
+    for (int v = 0; v < NV; ++v) at[v] = HALVES && skip[v] ? off[v] + back : off[v];
     if (policy.stream_loads) {
 #pragma unroll
-      for (int v = 0; v < NV; ++v) raw[v] = __builtin_amdgcn_raw_buffer_load_b128(r, off[v], 0, kAuxLoadStream);
+      for (int v = 0; v < NV; ++v) to.raw[v] = __builtin_amdgcn_raw_buffer_load_b128(r, at[v], 0, kAuxLoadStream);
     } else {
 #pragma unroll
-      for (int v = 0; v < NV; ++v) raw[v] = __builtin_amdgcn_raw_buffer_load_b128(r, off[v], 0, kAuxLoadCached);
+      for (int v = 0; v < NV; ++v) to.raw[v] = __builtin_amdgcn_raw_buffer_load_b128(r, at[v], 0, kAuxLoadCached);
+    }
+    if constexpr (HALVES) {
+      typedef const __attribute__((address_space(4))) uint32_t *Scalar;
+      const uintptr_t from = (reinterpret_cast<uintptr_t>(base) + (live ? row : 0u) * pitch) & ~(uintptr_t)3;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) to.more[v] = *reinterpret_cast<Scalar>(from + (back && live ? run_end(v) : 0u));
+    }
+  }
+  // Where the wave's run of vectors v ends, in bytes from the dword that a split row starts in; 0: it holds none.
+  // (The dword there holds the last element of the run's last vector.)
+  __device__ __forceinline__ unsigned run_end(int v) const {
+    const unsigned whole = cols / VE, from = (unsigned)v * size + (wave - index * waves) * 64u, end = from + 64u;
+    return from < whole ? (end < whole ? end : whole) * 16u : 0u;
+  }
+  __device__ __forceinline__ void settle(Loaded &l, const char *base, unsigned long long pitch, unsigned long long row) const {
+    if constexpr (HALVES) {
+      if (!split(base, pitch, row)) return;
+      // in the wave where the row ends there are lanes before the last whose next lane holds no neighbour
+      const unsigned whole = cols / VE;
+      const bool edge = ragged || (whole % 64u != 0 && (whole - 1u) % size / 64u == wave - index * waves);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const u32x4 a = l.raw[v];
+        // the next lane's first dword; the last lane keeps `more`, and lanes that hold nothing keep to zeros
+        const uint32_t more = run_end(v) ? l.more[v] : 0u;
+        uint32_t fifth = (uint32_t)__builtin_amdgcn_update_dpp((int)more, (int)a[0], kFromLaneBehind, 0xf, 0xf, false);
+        if (edge) fifth = off[v] == kNowhere ? 0u : vector(v) + 1u >= whole ? more : fifth;
+        u32x4 b;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = __builtin_amdgcn_alignbit(j < 3 ? a[j < 3 ? j + 1 : 3] : fifth, a[j], 16);
+        if (edge && skip[v]) b = a;
+        l.raw[v] = b;
+      }
     }
   }
   __device__ __forceinline__ void store(const u32x4 (&raw)[NV], char *base, unsigned long long pitch, unsigned long long row,

@@ -64,6 +64,10 @@ template <int VE> __device__ __forceinline__ float quotient_factor(float (&s)[VE
   return inv;
 }
 
+template <typename T, int NV, int VE> __device__ __forceinline__ void set_row(float (&s)[NV][VE], const u32x4 (&raw)[NV]) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v) Row<T>::unpack(s[v], raw[v]);
+}
 template <typename T, int NV, int VE> __device__ __forceinline__ void add_row(float (&s)[NV][VE], const u32x4 (&raw)[NV]) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
@@ -74,37 +78,36 @@ template <typename T, int NV, int VE> __device__ __forceinline__ void add_row(fl
   }
 }
 
-template <typename T, int NV, int VE> __device__ __forceinline__ void set_row(float (&s)[NV][VE], const u32x4 (&raw)[NV]) {
-#pragma unroll
-  for (int v = 0; v < NV; ++v) Row<T>::unpack(s[v], raw[v]);
-}
-
 // Adds streams [from, P) of a row to s, in rank order, the loads of B streams issued together.
-template <int B, typename T, int NV, int VE>
-__device__ __forceinline__ void add_streams(float (&s)[NV][VE], const RowTeam<T, NV> &team, const char *const *in, int from, int P,
+template <int B, typename T, int NV, int VE, bool HALVES>
+__device__ __forceinline__ void add_streams(float (&s)[NV][VE], const RowTeam<T, NV, HALVES> &team, const char *const *in, int from, int P,
                                             unsigned long long pitch, unsigned long long row, bool live) {
   for (int k = from; k < P; k += B) {
-    u32x4 raw[B][NV];
+    typename RowTeam<T, NV, HALVES>::Loaded got[B];
 #pragma unroll
     for (int b = 0; b < B; ++b)
-      if (k + b < P) team.load(raw[b], in[k + b], pitch, row, live);
+      if (k + b < P) team.load(got[b], in[k + b], pitch, row, live);
 #pragma unroll
     for (int b = 0; b < B; ++b)
-      if (k + b < P) add_row<T>(s, raw[b]);
+      if (k + b < P) {
+        team.settle(got[b], in[k + b], pitch, row);
+        add_row<T>(s, got[b].raw);
+      }
   }
 }
 
 // MANY: more than one rank.
-template <typename T, int NV, int OUT, bool MANY>
+template <typename T, int NV, int OUT, bool MANY, bool HALVES>
 __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
   constexpr int VE = Row<T>::VE;
   constexpr int B = NV >= 8 ? 1 : NV == 4 ? 2 : 4;
   __shared__ float lds[kMaxWaves * 2];
-  const RowTeam<T, NV> team(p.cols, p.shape, p.policy);
+  using Team = RowTeam<T, NV, HALVES>;
+  const Team team(p.cols, p.shape, p.policy);
   const unsigned long long row = (unsigned long long)blockIdx.x * p.shape.teams + team.index;
   const bool live = row < p.rows;
-  u32x4 raw[NV];
-  if (p.res) team.load(raw, p.res, p.res_pitch, row, live);
+  typename Team::Loaded res;
+  if (p.res) team.load(res, p.res, p.res_pitch, row, live);
   float s[NV][VE];
   if constexpr (MANY) {
 #pragma unroll
@@ -113,11 +116,16 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
       for (int j = 0; j < VE; ++j) s[v][j] = -0.0f;  // -0 + x is x, whatever x
     add_streams<B>(s, team, p.in, 0, p.P, p.in_pitch, row, live);
   } else {
-    u32x4 only[NV];
+    typename Team::Loaded only;
     team.load(only, p.in[0], p.in_pitch, row, live);
-    set_row<T>(s, only);
+    team.settle(only, p.in[0], p.in_pitch, row);
+    set_row<T>(s, only.raw);
   }
-  if (p.res) add_row<T>(s, raw);
+  if (p.res) {
+    team.settle(res, p.res, p.res_pitch, row);
+    add_row<T>(s, res.raw);
+  }
+  u32x4 raw[NV];
   float ss = 0.0f;
   if (team.ragged) {
 #pragma unroll
@@ -189,7 +197,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
       const float scale = scale_of(__builtin_fabsf(lanes_max(a, lanes) * rstd));
       // one lane of a group writes its scale; a group behind the row has no place among them
       const auto r = team.rsrc(reinterpret_cast<const char *>(p.scales), p.groups * 4u, row, live, p.groups * 4u);
-      const unsigned at = (team.lane & (lanes - 1)) == 0 ? (team.element(v) >> p.group_log2) * 4u : team.kNowhere;
+      const unsigned at = (team.lane & (lanes - 1)) == 0 ? (team.vector(v) * VE >> p.group_log2) * 4u : team.kNowhere;
       __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(scale), r, at, 0, 0);
       const float by = quotient_factor(s[v], rstd, scale);
       team.store_e4m3(s[v], v, by, p.apart, p.out, p.out_pitch, row, live);
@@ -252,9 +260,10 @@ struct GradParams {
 
 // What is read of a row up front: x, dsum, rstd and B of the ranks' gradients.
 template <typename T, int NV, int B> struct Fetched {
-  u32x4 x[NV], ds[NV], dy[B][NV];
+  using Team = RowTeam<T, NV, false>;
+  typename Team::Loaded x, ds, dy[B];
   float rstd;
-  __device__ __forceinline__ void fetch(const GradParams &p, const RowTeam<T, NV> &team, unsigned long long row) {
+  __device__ __forceinline__ void fetch(const GradParams &p, const Team &team, unsigned long long row) {
     const bool live = row < p.rows;
 #pragma unroll
     for (int b = 0; b < B; ++b)
@@ -272,7 +281,8 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
   constexpr bool AHEAD = !(WIDE || (NV == 2 && THREADS > 512));  // the next row is read ahead
   __shared__ float lds[2][kMaxWaves];
   extern __shared__ float4 kept[];  // WIDE: the weight's gradient; else room for half of the teams to hand it over
-  const RowTeam<T, NV> team(p.cols, p.shape, p.policy);
+  using Team = RowTeam<T, NV, false>;
+  const Team team(p.cols, p.shape, p.policy);
   auto slot = [&](int v, int j) -> float4 & { return kept[(unsigned)(v * (VE / 4) + j / 4) * team.size + team.lane]; };
   float dw[WIDE ? 1 : NV][VE], w[WIDE ? 1 : NV][VE];
   if constexpr (WIDE) {
@@ -304,17 +314,17 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
     // the next row's loads are on their way while this one's sum is made and its gradient written
     if constexpr (AHEAD) next.fetch(p, team, row + step);
     float g[NV][VE];
-    set_row<T>(g, now.dy[0]);
+    set_row<T>(g, now.dy[0].raw);
 #pragma unroll
     for (int b = 1; b < B; ++b)
-      if (b < p.P) add_row<T>(g, now.dy[b]);
+      if (b < p.P) add_row<T>(g, now.dy[b].raw);
     add_streams<(WIDE ? 1 : 4)>(g, team, p.dy, B, p.P, p.dy_pitch, row, live);
     float dot = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       if constexpr (NV >= 4) __builtin_amdgcn_sched_barrier(0);  // one vector after another: registers are short
       float x[VE], wv[VE], d[VE];
-      Row<T>::unpack(x, now.x[v]);
+      Row<T>::unpack(x, now.x.raw[v]);
       if constexpr (WIDE) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) wv[j] = 1.0f;
@@ -345,16 +355,16 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
       for (int v = 0; v < NV; ++v) {
         if constexpr (NV >= 4) __builtin_amdgcn_sched_barrier(0);
         float x[VE];
-        asm volatile("" : "+v"(now.x[v]));  // x is widened again, not kept as floats
-        Row<T>::unpack(x, now.x[v]);
+        asm volatile("" : "+v"(now.x.raw[v]));  // x is widened again, not kept as floats
+        Row<T>::unpack(x, now.x.raw[v]);
 #pragma unroll
         for (int j = 0; j < VE; ++j) g[v][j] = now.rstd * fmaf(-(x[j] * now.rstd), c, g[v][j]);
       }
       // (dsum was read before the team met: dx may take its place)
-      if (p.dsum) add_row<T>(g, now.ds);
+      if (p.dsum) add_row<T>(g, now.ds.raw);
 #pragma unroll
-      for (int v = 0; v < NV; ++v) now.x[v] = Row<T>::pack(g[v]);
-      team.store(now.x, p.dx, p.dx_pitch, row, live);
+      for (int v = 0; v < NV; ++v) now.x.raw[v] = Row<T>::pack(g[v]);
+      team.store(now.x.raw, p.dx, p.dx_pitch, row, live);
     }
   }
   if (!p.partial) return;
@@ -528,9 +538,17 @@ int check_common(int P, size_t cols, int dtype, const void *weight, int weight_d
 // Workgroups of a launch; what is left is done by further ones.
 constexpr size_t kMaxGrid = (size_t)1 << 21;
 
-// A call that moves less than this reads through the caches.
-constexpr size_t kStreamFromBytes = (size_t)256 << 20;
+// Whether rows of 16-bit elements may start in the middle of a dword.
+inline bool starts_in_a_dword(const void *at, size_t pitch) { return ((reinterpret_cast<uintptr_t>(at) | pitch) & 2u) != 0; }
+// Whether rows cover whole 64-byte pieces of memory.
+inline bool whole_lines(const void *at, size_t pitch, size_t bytes) {
+  return ((reinterpret_cast<uintptr_t>(at) | pitch | bytes) & 63u) == 0;
+}
 
+// A call that moves less than this reads through the caches.
+constexpr size_t kStreamFromBytes = (size_t)256 << 20, kGradStreamFromBytes = (size_t)64 << 20;
+
+// Waves that hold a row of `need` vectors, nv of them a lane.
 inline unsigned waves_for(unsigned need, unsigned nv) { return (need + 64 * nv - 1) / (64 * nv); }
 
 // The call on the rows from the first `done` on.
@@ -556,12 +574,21 @@ inline int launch_rows(void (*kern)(NormParams), const NormParams &p, size_t per
   return ALAMD_OK;
 }
 
-template <typename T, int NV> int launch_norm(NormParams &p, int out, unsigned waves, unsigned teams, hipStream_t stream) {
+template <typename T, int NV, bool MANY> void (*norm_kernel(int out, bool halves))(NormParams) {
+  if constexpr (sizeof(T) == 2)
+    if (halves)
+      return out == OUT_SAME       ? rms_norm_kernel<T, NV, OUT_SAME, MANY, true>
+             : out == OUT_E4M3_ROW ? rms_norm_kernel<T, NV, OUT_E4M3_ROW, MANY, true>
+                                   : rms_norm_kernel<T, NV, OUT_E4M3_GROUP, MANY, true>;
+  return out == OUT_SAME       ? rms_norm_kernel<T, NV, OUT_SAME, MANY, false>
+         : out == OUT_E4M3_ROW ? rms_norm_kernel<T, NV, OUT_E4M3_ROW, MANY, false>
+                               : rms_norm_kernel<T, NV, OUT_E4M3_GROUP, MANY, false>;
+}
+template <typename T, int NV>
+int launch_norm(NormParams &p, int out, bool halves, unsigned waves, unsigned teams, hipStream_t stream) {
   p.shape = {waves, teams};
-  auto kern = out == OUT_SAME ? (p.P > 1 ? rms_norm_kernel<T, NV, OUT_SAME, true> : rms_norm_kernel<T, NV, OUT_SAME, false>)
-              : out == OUT_E4M3_ROW ? (p.P > 1 ? rms_norm_kernel<T, NV, OUT_E4M3_ROW, true> : rms_norm_kernel<T, NV, OUT_E4M3_ROW, false>)
-              : (p.P > 1 ? rms_norm_kernel<T, NV, OUT_E4M3_GROUP, true> : rms_norm_kernel<T, NV, OUT_E4M3_GROUP, false>);
-  return launch_rows(kern, p, teams, 64 * waves * teams, stream);
+  return launch_rows(p.P > 1 ? norm_kernel<T, NV, true>(out, halves) : norm_kernel<T, NV, false>(out, halves), p, teams,
+                     64 * waves * teams, stream);
 }
 
 template <typename T> int norm_rows(NormParams &p, int out, hipStream_t stream) {
@@ -569,12 +596,18 @@ template <typename T> int norm_rows(NormParams &p, int out, hipStream_t stream) 
   if (p.cols < VE)
     return launch_rows(out == OUT_SAME ? rms_norm_short_kernel<T, false> : rms_norm_short_kernel<T, true>, p, 256, 256, stream);
   const unsigned need = (p.cols + VE - 1) / VE;  // vectors of a row
-  if (need <= 64) return launch_norm<T, 1>(p, out, 1, 4, stream);
-  if (p.rows <= 512 && need <= 1024) return launch_norm<T, 1>(p, out, waves_for(need, 1), 1, stream);
-  if (need <= 128) return launch_norm<T, 2>(p, out, 1, 4, stream);
-  if (need <= 2048) return launch_norm<T, 2>(p, out, waves_for(need, 2), 1, stream);
-  if (need <= 4096) return launch_norm<T, 4>(p, out, waves_for(need, 4), 1, stream);
-  if constexpr (VE == 4) return launch_norm<T, 8>(p, out, waves_for(need, 8), 1, stream);
+  bool halves = false;
+  if (sizeof(T) == 2) {
+    halves = p.res && starts_in_a_dword(p.res, p.res_pitch);
+    for (int k = 0; k < p.P; ++k) halves = halves || starts_in_a_dword(p.in[k], p.in_pitch);
+  }
+  const unsigned one = waves_for(need, 1), two = waves_for(need, 2), four = waves_for(need, 4);
+  if (one == 1) return launch_norm<T, 1>(p, out, halves, 1, 4, stream);
+  if (p.rows <= 512 && one <= kMaxWaves) return launch_norm<T, 1>(p, out, halves, one, 1, stream);
+  if (two == 1) return launch_norm<T, 2>(p, out, halves, 1, 4, stream);
+  if (two <= kMaxWaves) return launch_norm<T, 2>(p, out, halves, two, 1, stream);
+  if (four <= kMaxWaves) return launch_norm<T, 4>(p, out, halves, four, 1, stream);
+  if constexpr (sizeof(T) == 4) return launch_norm<T, 8>(p, out, halves, waves_for(need, 8), 1, stream);
   return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
 }
 
@@ -592,7 +625,8 @@ int launch_grad_b(GradParams &p, size_t *parts, unsigned waves, unsigned teams, 
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
-template <typename T, int NV, int THREADS> int launch_grad(GradParams &p, size_t *parts, unsigned waves, hipStream_t stream) {
+template <typename T, int NV, int THREADS>
+int launch_grad(GradParams &p, size_t *parts, unsigned waves, hipStream_t stream) {
   unsigned teams = THREADS / 64 / waves;
   while (teams > 1 && p.rows < (size_t)256 * teams) --teams;
   return p.P == 1 ? launch_grad_b<T, NV, 1, false, THREADS>(p, parts, waves, teams, stream)
@@ -610,11 +644,12 @@ template <typename T> int grad_rows(GradParams &p, size_t *parts, hipStream_t st
     return ALAMD_OK;
   }
   const unsigned need = (p.cols + VE - 1) / VE;
-  if (need <= 640) return launch_grad<T, 1, 1024>(p, parts, waves_for(need, 1), stream);
-  if (need <= 1024) return launch_grad<T, 2, 512>(p, parts, waves_for(need, 2), stream);
-  if (need <= 2048) return launch_grad_b<T, 2, 1, false, 1024>(p, parts, waves_for(need, 2), 1, stream);
-  if (need <= 4096) return launch_grad_b<T, 4, 1, true, 1024>(p, parts, waves_for(need, 4), 1, stream);
-  if constexpr (VE == 4) return launch_grad_b<T, 8, 1, true, 1024>(p, parts, waves_for(need, 8), 1, stream);
+  const unsigned one = waves_for(need, 1), two = waves_for(need, 2), four = waves_for(need, 4);
+  if (one <= 12) return launch_grad<T, 1, 1024>(p, parts, one, stream);
+  if (two <= 8) return launch_grad<T, 2, 512>(p, parts, two, stream);
+  if (two <= kMaxWaves) return launch_grad_b<T, 2, 1, false, 1024>(p, parts, two, 1, stream);
+  if (four <= kMaxWaves) return launch_grad_b<T, 4, 1, true, 1024>(p, parts, four, 1, stream);
+  if constexpr (sizeof(T) == 4) return launch_grad_b<T, 8, 1, true, 1024>(p, parts, waves_for(need, 8), 1, stream);
   return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
 }
 
@@ -677,9 +712,8 @@ int alamd_rms_norm(void *out, size_t out_stride, void *sum, const void *residual
   p.inv_n = 1.0f / (float)cols;
   p.apart = cols % (16 / es) != 0 && (cols - cols % (16 / es)) % (group ? group : cols) == 0;
   const size_t moved = rows * cols * (es * ((size_t)P + (residual ? 1 : 0) + (sum ? 1 : 0)) + oes);
-  const auto lines = [](const void *at, size_t pitch) { return ((reinterpret_cast<uintptr_t>(at) | pitch) & 63u) == 0; };
-  p.policy = {moved >= kStreamFromBytes,
-              moved >= kStreamFromBytes && lines(out, p.out_pitch) && (!sum || lines(sum, p.res_pitch))};
+  p.policy = {moved >= kStreamFromBytes, moved >= kStreamFromBytes && whole_lines(out, p.out_pitch, cols * oes) &&
+                                             (!sum || whole_lines(sum, p.res_pitch, cols * es))};
   const int kind = !scales ? OUT_SAME : group == 0 || group >= cols ? OUT_E4M3_ROW : OUT_E4M3_GROUP;
   switch (dtype) {
   case ALAMD_F16: return norm_rows<f16_t>(p, kind, as_stream(stream));
@@ -747,8 +781,8 @@ int alamd_rms_norm_grad(void *dx, size_t dx_stride, const void *const *dys, int 
     p.w32 = weight && weight_dtype == ALAMD_F32;
     p.inv_n = 1.0f / (float)cols;
     const size_t moved = rows * cols * es * ((size_t)P + 1 + (dsum ? 1 : 0) + (dx ? 1 : 0));
-    p.policy = {moved >= kStreamFromBytes,
-                moved >= kStreamFromBytes && ((reinterpret_cast<uintptr_t>(dx) | p.dx_pitch) & 63u) == 0};
+    p.policy = {moved >= kGradStreamFromBytes,
+                moved >= kGradStreamFromBytes && whole_lines(dx, p.dx_pitch, cols * es)};
     switch (dtype) {
     case ALAMD_F16: rc = grad_rows<f16_t>(p, &parts, as_stream(stream)); break;
     case ALAMD_BF16: rc = grad_rows<bf16_t>(p, &parts, as_stream(stream)); break;
