@@ -157,7 +157,8 @@ def _infer_dtype(t):
 def _stream(stream):
     import torch
     if stream is None:
-        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        # (torch.cuda.current_stream() builds an object: 2.7 us against 0.2)
+        return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
     if isinstance(stream, int):
         return C.c_void_p(stream)
     return C.c_void_p(stream.cuda_stream)
@@ -357,45 +358,77 @@ def copy(dst, src, nbytes=None, stream=None):
                              _stream(stream)))
 
 
-def _on_device(t):
+_TYPE_CODES = {}
+
+
+def _type_code(dtype):
+    """Library number of a torch dtype that rows of the operators below may have; None for others."""
+    if not _TYPE_CODES:
+        import torch
+        _TYPE_CODES.update({torch.float16: DTYPES.index("f16"), torch.bfloat16: DTYPES.index("bf16"),
+                            torch.float32: DTYPES.index("f32")})
+    return _TYPE_CODES.get(dtype)
+
+
+def _device_of(t):
+    """The device of a tensor, which has to be the current one."""
     import torch
-    if not t.is_cuda:
+    dev = t.get_device()
+    if dev < 0:
         raise AlError(1, "buffers must live on the GPU")
-    if t.get_device() != torch.cuda.current_device():
-        raise AlError(1, "a buffer lives on device %d, the current device is %d" % (t.get_device(), torch.cuda.current_device()))
+    if dev != torch.cuda.current_device():
+        raise AlError(1, "a buffer lives on device %d, the current device is %d" % (dev, torch.cuda.current_device()))
+    return dev
 
 
-def _matrix(t, shape, dtype, what):
+def _same_device(t, dev):
+    if t.get_device() != dev:
+        raise AlError(1, "buffers must live on the GPU" if t.get_device() < 0 else
+                      "a buffer lives on device %d, another one on device %d" % (t.get_device(), dev))
+
+
+def _matrix(t, shape, dtype, dev, what):
     """(address, elements between rows) of a matrix on the GPU whose rows are contiguous."""
     if t.shape != shape or t.dtype != dtype:
         raise AlError(1, "%s is %s of %s, expected %s of %s" % (what, tuple(t.shape), t.dtype, tuple(shape), dtype))
-    _on_device(t)
+    if t.get_device() != dev:
+        _same_device(t, dev)
     row, col = t.stride()
     if col != 1 and shape[1] > 1:
         raise AlError(1, "rows must be contiguous")
-    return t.data_ptr(), (row if shape[0] > 1 else max(row, shape[1]))
+    if row < shape[1]:
+        # (a single row may have any stride)
+        if shape[0] > 1:
+            raise AlError(1, "rows of %s lie %d elements apart and are %d long" % (what, row, shape[1]))
+        row = shape[1]
+    return t.data_ptr(), row
 
 
-def _vector(t, n, dtype, what):
+def _vector(t, n, dtype, dev, what):
     """Address of n contiguous elements on the GPU, of any shape."""
     if t.numel() != n or t.dtype != dtype:
         raise AlError(1, "%s has %d elements of %s, expected %d of %s" % (what, t.numel(), t.dtype, n, dtype))
-    _on_device(t)
+    if t.get_device() != dev:
+        _same_device(t, dev)
     if not t.is_contiguous():
         raise AlError(1, "buffers must be contiguous")
     return t.data_ptr()
 
 
-def _rank_matrices(tensors, shape, dtype, what):
+def _rank_matrices(tensors, shape, dtype, dev, what):
     """Table of the ranks' matrices, which share one distance between rows, and that distance."""
-    arr = (C.c_void_p * len(tensors))()
-    stride = None
-    for k, t in enumerate(tensors):
-        arr[k], s = _matrix(t, shape, dtype, what)
-        if stride is not None and s != stride:
-            raise AlError(1, "%s of every rank must have the same distance between rows" % what)
-        stride = s
-    return arr, stride
+    first, stride = _matrix(tensors[0], shape, dtype, dev, what)
+    like = tensors[0].stride()
+    at = [first]
+    for t in tensors[1:]:
+        if t.shape != shape or t.dtype != dtype or t.get_device() != dev or t.stride() != like:
+            p, s = _matrix(t, shape, dtype, dev, what)
+            if s != stride and shape[0] > 1:
+                raise AlError(1, "%s of every rank must have the same distance between rows" % what)
+            at.append(p)
+        else:
+            at.append(t.data_ptr())
+    return (C.c_void_p * len(at))(*at), stride
 
 
 def rms_norm(out, ins, weight=None, residual=None, sum_out=None, rstd=None, scales=None, group=0, eps=1e-6, stream=None):
@@ -406,35 +439,36 @@ def rms_norm(out, ins, weight=None, residual=None, sum_out=None, rstd=None, scal
     x = ins[0]
     if x.dim() != 2:
         raise AlError(1, "rms_norm takes matrices of [rows, cols]")
-    shape, dtype = x.shape, x.dtype
+    shape, dtype, dev = x.shape, x.dtype, _device_of(x)
     rows, cols = shape
-    table, in_stride = _rank_matrices(ins, shape, dtype, "a rank's input")
-    out_p, out_stride = _matrix(out, shape, dtype if scales is None else torch.float8_e4m3fn, "out")
+    code = _type_code(dtype)
+    if code is None:
+        raise AlError(3, "a norm takes float16, bfloat16 or float32 rows, not %s" % dtype)
+    table, in_stride = _rank_matrices(ins, shape, dtype, dev, "a rank's input")
+    out_p, out_stride = _matrix(out, shape, dtype if scales is None else torch.float8_e4m3fn, dev, "out")
     res_p = sum_p = None
     res_stride = 0
     if residual is not None:
-        res_p, res_stride = _matrix(residual, shape, dtype, "residual")
+        res_p, res_stride = _matrix(residual, shape, dtype, dev, "residual")
     if sum_out is not None:
-        sum_p, s = _matrix(sum_out, shape, dtype, "sum_out")
-        if residual is not None and s != res_stride:
+        sum_p, s = _matrix(sum_out, shape, dtype, dev, "sum_out")
+        if residual is not None and s != res_stride and rows > 1:
             raise AlError(1, "residual and sum_out must have the same distance between rows")
         res_stride = s
-    w_p, w_dt = _weight(weight, cols, dtype)
+    w_p, w_dt = (None, code) if weight is None else _weight(weight, cols, dtype, dev)
     groups = -(-cols // group) if group > 0 else 1
     _check(load().alamd_rms_norm(
         out_p, out_stride, sum_p, res_p, res_stride, table, len(ins), in_stride, w_p, w_dt,
-        None if rstd is None else _vector(rstd, rows, torch.float32, "rstd"),
-        None if scales is None else _vector(scales, rows * groups, torch.float32, "scales"),
-        group, rows, cols, DTYPES.index(_infer_dtype(x)), eps, _stream(stream)))
+        None if rstd is None else _vector(rstd, rows, torch.float32, dev, "rstd"),
+        None if scales is None else _vector(scales, rows * groups, torch.float32, dev, "scales"),
+        group, rows, cols, code, eps, _stream(stream)))
 
 
-def _weight(weight, cols, dtype):
+def _weight(weight, cols, dtype, dev):
     import torch
-    if weight is None:
-        return None, DTYPES.index("f32")
     if weight.dtype != dtype and weight.dtype != torch.float32:
         raise AlError(3, "the weight has the rows' type or float32, not %s" % weight.dtype)
-    return _vector(weight, cols, weight.dtype, "weight"), DTYPES.index(_infer_dtype(weight))
+    return _vector(weight, cols, weight.dtype, dev, "weight"), _type_code(weight.dtype)
 
 
 def rms_norm_grad_workspace(rows, cols):
@@ -449,28 +483,31 @@ def rms_norm_grad(dx, dys, x, rstd, weight=None, dsum=None, dweight=None, worksp
     import torch
     if x.dim() != 2:
         raise AlError(1, "rms_norm_grad takes matrices of [rows, cols]")
-    shape, dtype = x.shape, x.dtype
+    shape, dtype, dev = x.shape, x.dtype, _device_of(x)
     rows, cols = shape
-    table, dy_stride = _rank_matrices(dys, shape, dtype, "a rank's gradient")
-    x_p, x_stride = _matrix(x, shape, dtype, "x")
-    dx_p, dx_stride = (None, cols) if dx is None else _matrix(dx, shape, dtype, "dx")
-    ds_p, ds_stride = (None, cols) if dsum is None else _matrix(dsum, shape, dtype, "dsum")
-    w_p, w_dt = _weight(weight, cols, dtype)
+    code = _type_code(dtype)
+    if code is None:
+        raise AlError(3, "a norm takes float16, bfloat16 or float32 rows, not %s" % dtype)
+    table, dy_stride = _rank_matrices(dys, shape, dtype, dev, "a rank's gradient")
+    x_p, x_stride = _matrix(x, shape, dtype, dev, "x")
+    dx_p, dx_stride = (None, cols) if dx is None else _matrix(dx, shape, dtype, dev, "dx")
+    ds_p, ds_stride = (None, cols) if dsum is None else _matrix(dsum, shape, dtype, dev, "dsum")
+    w_p, w_dt = (None, code) if weight is None else _weight(weight, cols, dtype, dev)
     dw_p = ws_p = None
     if dweight is not None:
         if weight is None:
-            w_dt = _weight(dweight, cols, dtype)[1]
-        dw_p = _vector(dweight, cols, dweight.dtype if weight is None else weight.dtype, "dweight")
+            dw_p, w_dt = _weight(dweight, cols, dtype, dev)
+        else:
+            dw_p = _vector(dweight, cols, weight.dtype, dev, "dweight")
         if rows:
             need = rms_norm_grad_workspace(rows, cols)
             have = 0 if workspace is None else workspace.numel() * workspace.element_size()
             if have < need:
                 raise AlError(1, "dweight needs a workspace of %d bytes, not %d" % (need, have))
-            ws_p = _vector(workspace, workspace.numel(), workspace.dtype, "workspace")
+            ws_p = _vector(workspace, workspace.numel(), workspace.dtype, dev, "workspace")
     _check(load().alamd_rms_norm_grad(
         dx_p, dx_stride, table, len(dys), dy_stride, x_p, x_stride, ds_p, ds_stride,
-        _vector(rstd, rows, torch.float32, "rstd"), w_p, w_dt, dw_p, rows, cols, DTYPES.index(_infer_dtype(x)), ws_p,
-        _stream(stream)))
+        _vector(rstd, rows, torch.float32, dev, "rstd"), w_p, w_dt, dw_p, rows, cols, code, ws_p, _stream(stream)))
 
 
 class TensorList:
@@ -485,8 +522,9 @@ class TensorList:
         self._h = C.c_void_p(None)
         self._keep = (list(ins), None if outs is None else list(outs))
         n = len(self._keep[0])
+        self._dev = _device_of(self._keep[0][0]) if n else torch.cuda.current_device()
         for t in self._keep[0] + (self._keep[1] or []):
-            _on_device(t)
+            _same_device(t, self._dev)
         if outs is not None:
             if len(self._keep[1]) != n:
                 raise AlError(1, "%d outputs for %d tensors" % (len(self._keep[1]), n))
@@ -500,27 +538,28 @@ class TensorList:
         self._workspace = torch.empty(self.WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
 
     def _space(self, workspace):
-        w = self._workspace if workspace is None else workspace
-        if w.numel() * w.element_size() < self.WORKSPACE_BYTES:
+        if workspace is None:
+            return self._workspace.data_ptr()
+        if workspace.numel() * workspace.element_size() < self.WORKSPACE_BYTES:
             raise AlError(1, "the workspace has less than %d bytes" % self.WORKSPACE_BYTES)
-        return _vector(w, w.numel(), w.dtype, "workspace")
+        return _vector(workspace, workspace.numel(), workspace.dtype, self._dev, "workspace")
+
+    def _norm(self, norm):
+        import torch
+        return _vector(norm, 1, torch.float32, self._dev, "norm")
 
     def global_norm(self, norm, workspace=None, stream=None):
         """norm[0] = the norm over all elements (alamd_global_norm)."""
-        import torch
-        _check(load().alamd_global_norm(self._h, _vector(norm, 1, torch.float32, "norm"), self._space(workspace),
-                                        _stream(stream)))
+        _check(load().alamd_global_norm(self._h, self._norm(norm), self._space(workspace), _stream(stream)))
 
     def clip_to_norm(self, norm, max_norm, eps=1e-6, stream=None):
         """Scales by max_norm / (norm[0] + eps) where that is below 1 (alamd_clip_to_norm)."""
-        import torch
-        _check(load().alamd_clip_to_norm(self._h, _vector(norm, 1, torch.float32, "norm"), max_norm, eps, _stream(stream)))
+        _check(load().alamd_clip_to_norm(self._h, self._norm(norm), max_norm, eps, _stream(stream)))
 
     def clip_global_norm(self, norm, max_norm, eps=1e-6, workspace=None, stream=None):
         """Both (alamd_clip_global_norm)."""
-        import torch
-        _check(load().alamd_clip_global_norm(self._h, _vector(norm, 1, torch.float32, "norm"), max_norm, eps,
-                                             self._space(workspace), _stream(stream)))
+        _check(load().alamd_clip_global_norm(self._h, self._norm(norm), max_norm, eps, self._space(workspace),
+                                             _stream(stream)))
 
     def destroy(self):
         if self._h:
