@@ -31,6 +31,7 @@ struct Chunk {
 struct alamd_tensor_list {
   int device;
   size_t chunks;
+  size_t bytes;
   alamd::Chunk *table;  // in device memory
 };
 
@@ -38,85 +39,147 @@ namespace alamd {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kU = 4;  // vectors a lane has under way (2 or 8: up to 3 % slower)
 constexpr size_t kChunkBytes = (size_t)64 << 10;
+// Norm and clipping in one call read a list of up to this size through the caches, whose memory-side 256 MiB then hold
+// most of it for the second pass; a longer one past them (us, through / past: lists of 30 MiB 17.9 / 21.7, 207 MiB
+// 108 / 117, 272 MiB 140 / 150, 1.3 GiB 747 / 687; keeping the last 64 to 224 MiB of that: 682 to 708).
+constexpr size_t kCachedBytes = (size_t)288 << 20;
 constexpr size_t kParts = ALAMD_GLOBAL_NORM_WORKSPACE_BYTES / sizeof(double);
 
 // ---- norm -------------------------------------------------------------------
 
-template <typename T> __device__ __forceinline__ double chunk_squares(const Chunk &c) {
+template <typename T> __device__ __forceinline__ double square_of(const char *at, unsigned e) {
+  const double x = (double)Row<T>::get(at, e);
+  return x * x;
+}
+
+// The squares of a chunk, this lane's part.
+template <typename T, int AUX> __device__ __forceinline__ double chunk_squares(const Chunk &c) {
   constexpr unsigned VE = Row<T>::VE;
-  const unsigned vecs = c.count / VE;
+  const unsigned head = (unsigned)head_count(sizeof(T), c.in, c.in, c.count), vecs = (c.count - head) / VE;
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(c.in + head * sizeof(T)), 0, (int)(vecs * 16u), kRsrcFlags);
   double a = 0.0;
-  for (unsigned i = threadIdx.x; i < vecs; i += kThreads) {
-    float x[VE];
-    Row<T>::unpack(x, *reinterpret_cast<const u32x4 *>(c.in + (size_t)i * 16));
+  for (unsigned i = threadIdx.x; i < vecs + threadIdx.x; i += kThreads * kU) {
+    u32x4 raw[kU];  // behind the last vector: zeros
 #pragma unroll
-    for (unsigned j = 0; j < VE; ++j) a = fma((double)x[j], (double)x[j], a);
+    for (int u = 0; u < kU; ++u) raw[u] = __builtin_amdgcn_raw_buffer_load_b128(r, (i + (unsigned)u * kThreads) * 16u, 0, AUX);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float x[VE];
+      Row<T>::unpack(x, raw[u]);
+#pragma unroll
+      for (unsigned j = 0; j < VE; ++j) a = fma((double)x[j], (double)x[j], a);
+    }
   }
-  const unsigned e = vecs * VE + threadIdx.x;
-  if (e < c.count) {
-    const double x = (double)Row<T>::get(c.in, e);
-    a = fma(x, x, a);
-  }
+  // the elements in front of the first 64-byte boundary and behind the last vector
+  if (threadIdx.x < head) a += square_of<T>(c.in, threadIdx.x);
+  const unsigned e = head + vecs * VE + threadIdx.x;
+  if (e < c.count) a += square_of<T>(c.in, e);
   return a;
 }
 
 // The sum over the workgroup, in every lane.
-template <int THREADS> __device__ __forceinline__ double block_sum(double a) {
-  __shared__ double lds[THREADS / 64];
+__device__ __forceinline__ double block_sum(double a) {
+  __shared__ double lds[kThreads / 64];
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) a += __shfl_xor(a, d);
   if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = a;
   __syncthreads();
   a = lds[0];
 #pragma unroll
-  for (int k = 1; k < THREADS / 64; ++k) a += lds[k];
+  for (int k = 1; k < kThreads / 64; ++k) a += lds[k];
   return a;
 }
 
+template <int AUX> __device__ __forceinline__ double chunk_squares(const Chunk &c) {
+  return c.dtype == ALAMD_F32    ? chunk_squares<float, AUX>(c)
+         : c.dtype == ALAMD_BF16 ? chunk_squares<bf16_t, AUX>(c)
+                                 : chunk_squares<f16_t, AUX>(c);
+}
+
+template <int AUX>
 __global__ void __launch_bounds__(kThreads) squares_kernel(const Chunk *table, unsigned long long chunks, double *parts) {
   double a = 0.0;
+  Chunk next = table[blockIdx.x];
   for (unsigned long long k = blockIdx.x; k < chunks; k += gridDim.x) {
-    const Chunk c = table[k];
-    a += c.dtype == ALAMD_F32 ? chunk_squares<float>(c) : c.dtype == ALAMD_BF16 ? chunk_squares<bf16_t>(c) : chunk_squares<f16_t>(c);
+    const Chunk c = next;
+    next = table[k + gridDim.x < chunks ? k + gridDim.x : k];
+    a += chunk_squares<AUX>(c);
   }
-  a = block_sum<kThreads>(a);
+  a = block_sum(a);
   if (threadIdx.x == 0) parts[blockIdx.x] = a;
 }
 
-__global__ void __launch_bounds__(kThreads) norm_kernel(const double *parts, unsigned n, float *norm) {
+// The norm from the workgroups' parts, in every lane of a workgroup.
+__device__ __forceinline__ float norm_of_parts(const double *parts, unsigned n) {
   double a = 0.0;
-  for (unsigned k = threadIdx.x; k < n; k += kThreads) a += parts[k];
-  a = block_sum<kThreads>(a);
-  if (threadIdx.x == 0) *norm = (float)sqrt(a);
+  for (unsigned k = threadIdx.x; k < n; k += kThreads * 8) {
+    double x[8];
+#pragma unroll
+    for (unsigned u = 0; u < 8; ++u) x[u] = k + u * kThreads < n ? parts[k + u * kThreads] : 0.0;
+#pragma unroll
+    for (unsigned u = 0; u < 8; ++u) a += x[u];
+  }
+  return (float)sqrt(block_sum(a));
+}
+
+__global__ void __launch_bounds__(kThreads) norm_kernel(const double *parts, unsigned n, float *norm) {
+  const float x = norm_of_parts(parts, n);
+  if (threadIdx.x == 0) *norm = x;
 }
 
 // ---- clipping ---------------------------------------------------------------
 
-template <typename T> __device__ __forceinline__ void chunk_scale(const Chunk &c, float by) {
+template <typename T, int AUX> __device__ __forceinline__ void chunk_scale(const Chunk &c, float by) {
   constexpr unsigned VE = Row<T>::VE;
-  const unsigned vecs = c.count / VE;
-  for (unsigned i = threadIdx.x; i < vecs; i += kThreads) {
-    float x[VE];
-    Row<T>::unpack(x, *reinterpret_cast<const u32x4 *>(c.in + (size_t)i * 16));
+  const unsigned head = (unsigned)head_count(sizeof(T), c.out, c.in, c.count), vecs = (c.count - head) / VE;
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(c.in + head * sizeof(T)), 0, (int)(vecs * 16u), kRsrcFlags);
+  const auto w = __builtin_amdgcn_make_buffer_rsrc(c.out + head * sizeof(T), 0, (int)(vecs * 16u), kRsrcFlags);
+  for (unsigned i = threadIdx.x; i < vecs + threadIdx.x; i += kThreads * kU) {
+    u32x4 raw[kU];
 #pragma unroll
-    for (unsigned j = 0; j < VE; ++j) x[j] *= by;
-    *reinterpret_cast<u32x4 *>(c.out + (size_t)i * 16) = Row<T>::pack(x);
+    for (int u = 0; u < kU; ++u) raw[u] = __builtin_amdgcn_raw_buffer_load_b128(r, (i + (unsigned)u * kThreads) * 16u, 0, AUX);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float x[VE];
+      Row<T>::unpack(x, raw[u]);
+#pragma unroll
+      for (unsigned j = 0; j < VE; ++j) x[j] *= by;
+      __builtin_amdgcn_raw_buffer_store_b128(Row<T>::pack(x), w, (i + (unsigned)u * kThreads) * 16u, 0, kAuxStoreRow);
+    }
   }
-  const unsigned e = vecs * VE + threadIdx.x;
+  if (threadIdx.x < head) Row<T>::put(c.out, threadIdx.x, Row<T>::get(c.in, threadIdx.x) * by);
+  const unsigned e = head + vecs * VE + threadIdx.x;
   if (e < c.count) Row<T>::put(c.out, e, Row<T>::get(c.in, e) * by);
 }
 
-__global__ void __launch_bounds__(kThreads) clip_kernel(const Chunk *table, unsigned long long chunks, const float *norm,
-                                                        float max_norm, float eps) {
-  const float n = *norm + eps;
-  const float by = n <= max_norm ? 1.0f : max_norm / n;
+template <int AUX> __device__ __forceinline__ void chunk_scale(const Chunk &c, float by) {
+  if (c.dtype == ALAMD_F32) chunk_scale<float, AUX>(c, by);
+  else if (c.dtype == ALAMD_BF16) chunk_scale<bf16_t, AUX>(c, by);
+  else chunk_scale<f16_t, AUX>(c, by);
+}
+
+// Clips to the norm in *norm, or, with `parts`, to the norm that those make, which the first workgroup writes to
+// *norm.  From the last chunk to the first: what the pass before has read last is the likeliest to be in a cache.
+template <bool PARTS, int AUX>
+__global__ void __launch_bounds__(kThreads) clip_kernel(const Chunk *table, unsigned long long chunks, const double *parts, unsigned n,
+                                                        float *norm, float max_norm, float eps) {
+  Chunk next = table[chunks - 1 - blockIdx.x];
+  float total;
+  if constexpr (PARTS) {
+    total = norm_of_parts(parts, n);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
+  } else {
+    total = *norm;
+  }
+  total += eps;
+  const float by = total <= max_norm ? 1.0f : max_norm / total;
   for (unsigned long long k = blockIdx.x; k < chunks; k += gridDim.x) {
-    const Chunk c = table[k];
+    const Chunk c = next;
+    next = table[k + gridDim.x < chunks ? chunks - 1 - k - gridDim.x : 0];
     if (by == 1.0f && c.in == c.out) continue;  // nothing to clip
-    if (c.dtype == ALAMD_F32) chunk_scale<float>(c, by);
-    else if (c.dtype == ALAMD_BF16) chunk_scale<bf16_t>(c, by);
-    else chunk_scale<f16_t>(c, by);
+    chunk_scale<AUX>(c, by);
   }
 }
 
@@ -139,22 +202,33 @@ int check_clip(const float *norm, float max_norm, float eps) {
   return ALAMD_OK;
 }
 
-int launch_norm(const alamd_tensor_list *list, float *norm, void *workspace, hipStream_t stream) {
-  const unsigned parts = (unsigned)(list->chunks < kParts ? list->chunks : kParts);
-  double *sums = static_cast<double *>(workspace);
-  if (parts) hipLaunchKernelGGL(squares_kernel, dim3(parts), dim3(kThreads), 0, stream, list->table, list->chunks, sums);
-  hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, stream, sums, parts, norm);
+// Workgroups of a pass; one that has done its chunk takes the next one that far on.  The norm runs at the rate of a large
+// copy with four or two workgroups a CU (847 MB of bf16: 130 us, 6.5 TB/s; eight a CU 136 us); the clipping likes one
+// chunk a workgroup (2.8 GB read and written after the norm: 687 us; 2048 workgroups 718 us).
+constexpr size_t kNormGrid = 1024, kClipGrid = (size_t)1 << 16;
+static_assert(kNormGrid <= kParts, "the workspace holds a part of every workgroup");
+
+unsigned launch_squares(const alamd_tensor_list *list, bool cached, double *parts, hipStream_t stream) {
+  const unsigned grid = (unsigned)(list->chunks < kNormGrid ? list->chunks : kNormGrid);
+  if (grid)
+    hipLaunchKernelGGL(cached ? squares_kernel<kAuxLoadCached> : squares_kernel<kAuxLoadStream>, dim3(grid), dim3(kThreads), 0, stream,
+                       list->table, list->chunks, parts);
+  return grid;
+}
+
+int launch_norm(const alamd_tensor_list *list, float *norm, double *parts, hipStream_t stream) {
+  const unsigned n = launch_squares(list, false, parts, stream);
+  hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, stream, parts, n, norm);
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
 
-// Workgroups of a clipping launch: a workgroup that has done its chunk takes the next one that far on.
-constexpr size_t kMaxClipGrid = (size_t)1 << 20;
-
-int launch_clip(const alamd_tensor_list *list, const float *norm, float max_norm, float eps, hipStream_t stream) {
-  if (list->chunks == 0) return ALAMD_OK;
-  const unsigned grid = (unsigned)(list->chunks < kMaxClipGrid ? list->chunks : kMaxClipGrid);
-  hipLaunchKernelGGL(clip_kernel, dim3(grid), dim3(kThreads), 0, stream, list->table, list->chunks, norm, max_norm, eps);
+int launch_clip(const alamd_tensor_list *list, bool cached, const double *parts, unsigned n, float *norm, float max_norm, float eps,
+                hipStream_t stream) {
+  const unsigned grid = (unsigned)(list->chunks < kClipGrid ? list->chunks : kClipGrid);
+  auto kern = !parts ? clip_kernel<false, kAuxLoadStream>
+              : cached ? clip_kernel<true, kAuxLoadCached> : clip_kernel<true, kAuxLoadStream>;
+  if (grid) hipLaunchKernelGGL(kern, dim3(grid), dim3(kThreads), 0, stream, list->table, list->chunks, parts, n, norm, max_norm, eps);
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
@@ -181,10 +255,14 @@ int make_chunks(std::vector<Chunk> &table, void *const *outs, const void *const 
     if (counts[t] > ((size_t)1 << 46) / es) return set_error(ALAMD_ERR_INVALID_ARG, "tensor %zu is too large", t);
     const uintptr_t at = reinterpret_cast<uintptr_t>(out);
     written.push_back({at, at + counts[t] * es, t});
-    const size_t per = kChunkBytes / es;
-    for (size_t e = 0; e < counts[t]; e += per) {
-      const size_t left = counts[t] - e;
-      table.push_back({in + e * es, out + e * es, (unsigned)(left < per ? left : per), dtypes[t]});
+    // the first chunk ends on a 64-byte boundary of the output (of the input, where they lie apart by no whole
+    // number of dwords), so that all others start on one
+    const size_t per = kChunkBytes / es, head = head_count(es, out, in, counts[t]);
+    for (size_t e = 0; e < counts[t];) {
+      const size_t left = counts[t] - e, most = e == 0 && head ? per - 64 / es + head : per;
+      const size_t count = left < most ? left : most;
+      table.push_back({in + e * es, out + e * es, (unsigned)count, dtypes[t]});
+      e += count;
     }
   }
   // what is written is written once, and read by its own tensor alone
@@ -218,7 +296,8 @@ int alamd_tensor_list_create(alamd_tensor_list **list, void *const *outs, const 
   try {
     std::vector<Chunk> table;
     if (int rc = make_chunks(table, outs, ins, counts, dtypes, n)) return rc;
-    std::unique_ptr<alamd_tensor_list> made(new alamd_tensor_list{0, table.size(), nullptr});
+    std::unique_ptr<alamd_tensor_list> made(new alamd_tensor_list{0, table.size(), 0, nullptr});
+    for (const Chunk &c : table) made->bytes += c.count * alamd_dtype_size(c.dtype);
     ALAMD_HIP(hipGetDevice(&made->device));
     if (!table.empty()) {
       ALAMD_HIP(hipMalloc(reinterpret_cast<void **>(&made->table), table.size() * sizeof(Chunk)));
@@ -247,13 +326,13 @@ int alamd_global_norm(const alamd_tensor_list *list, float *norm, void *workspac
   if (int rc = check_list(list)) return rc;
   if (int rc = check_clip(norm, 0.0f, 0.0f)) return rc;
   if (int rc = check_workspace(workspace)) return rc;
-  return launch_norm(list, norm, workspace, as_stream(stream));
+  return launch_norm(list, norm, static_cast<double *>(workspace), as_stream(stream));
 }
 
 int alamd_clip_to_norm(const alamd_tensor_list *list, const float *norm, float max_norm, float eps, void *stream) {
   if (int rc = check_list(list)) return rc;
   if (int rc = check_clip(norm, max_norm, eps)) return rc;
-  return launch_clip(list, norm, max_norm, eps, as_stream(stream));
+  return launch_clip(list, false, nullptr, 0, const_cast<float *>(norm), max_norm, eps, as_stream(stream));
 }
 
 int alamd_clip_global_norm(const alamd_tensor_list *list, float *norm, float max_norm, float eps, void *workspace,
@@ -261,8 +340,11 @@ int alamd_clip_global_norm(const alamd_tensor_list *list, float *norm, float max
   if (int rc = check_list(list)) return rc;
   if (int rc = check_clip(norm, max_norm, eps)) return rc;
   if (int rc = check_workspace(workspace)) return rc;
-  if (int rc = launch_norm(list, norm, workspace, as_stream(stream))) return rc;
-  return launch_clip(list, norm, max_norm, eps, as_stream(stream));
+  double *parts = static_cast<double *>(workspace);
+  if (list->chunks == 0) return launch_norm(list, norm, parts, as_stream(stream));
+  const bool cached = list->bytes <= kCachedBytes;
+  const unsigned n = launch_squares(list, cached, parts, as_stream(stream));
+  return launch_clip(list, cached, parts, n, norm, max_norm, eps, as_stream(stream));
 }
 
 }  // extern "C"
