@@ -11,6 +11,7 @@
 //
 // Backward, from the saved sum x and rstd, with dy = dy_0 + .. + dy_{P-1}, n_hat = x * rstd, g = dy * w:
 //   dx = rstd * (g - n_hat * sum(g * n_hat) / n) (+ dsum),   dw = sum over rows of dy * n_hat
+// with the factors of a row gathered: dx = rstd * (g - m * x) + dsum, m = rstd * sum(g * n_hat) / n.
 //
 // A team of TEAM lanes holds a row in registers: NV 128-bit vectors per lane and stream, read once.  The
 // elements behind the last whole vector belong to the next lane, whose vector is moved back so that it ends with
@@ -100,7 +101,7 @@ __device__ __forceinline__ void add_streams(float (&s)[NV][VE], const RowTeam<T,
 template <typename T, int NV, int OUT, bool MANY, bool HALVES>
 __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
   constexpr int VE = Row<T>::VE;
-  constexpr int B = NV >= 8 ? 1 : NV == 4 ? 2 : 4;
+  constexpr int B = NV >= 8 ? 1 : NV >= 3 ? 2 : 4;
   __shared__ float lds[kMaxWaves * 2];
   using Team = RowTeam<T, NV, HALVES>;
   const Team team(p.cols, p.shape, p.policy);
@@ -337,12 +338,18 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
       }
 #pragma unroll
       for (int j = 0; j < VE; ++j) {
-        const float n = x[j] * now.rstd;
+        x[j] *= now.rstd;
         // a row that is not there has rstd = 0 and reads zeros
-        if constexpr (WIDE) d[j] = fmaf(g[v][j], n, d[j]);
-        else dw[v][j] = fmaf(g[v][j], n, dw[v][j]);
+        if constexpr (WIDE) d[j] = fmaf(g[v][j], x[j], d[j]);
+        else dw[v][j] = fmaf(g[v][j], x[j], dw[v][j]);
         g[v][j] *= WIDE ? wv[j] : w[WIDE ? 0 : v][j];
-        dot = fmaf(g[v][j], !team.ragged || team.counts(v, j) ? n : 0.0f, dot);
+      }
+      if (team.ragged) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) dot = fmaf(g[v][j], team.counts(v, j) ? x[j] : 0.0f, dot);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) dot = fmaf(g[v][j], x[j], dot);
       }
       if constexpr (WIDE) {
 #pragma unroll
@@ -350,7 +357,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
       }
     }
     if (p.dx) {
-      const float c = team.sum(dot, lds[turn]) * p.inv_n;
+      const float m = team.sum(dot, lds[turn]) * p.inv_n * now.rstd;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         if constexpr (NV >= 4) __builtin_amdgcn_sched_barrier(0);
@@ -358,12 +365,19 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
         asm volatile("" : "+v"(now.x.raw[v]));  // x is widened again, not kept as floats
         Row<T>::unpack(x, now.x.raw[v]);
 #pragma unroll
-        for (int j = 0; j < VE; ++j) g[v][j] = now.rstd * fmaf(-(x[j] * now.rstd), c, g[v][j]);
-      }
-      // (dsum was read before the team met: dx may take its place)
-      if (p.dsum) add_row<T>(g, now.ds.raw);
+        for (int j = 0; j < VE; ++j) g[v][j] = fmaf(-m, x[j], g[v][j]);
+        // (dsum was read before the team met: dx may take its place)
+        if (p.dsum) {
+          float d[VE];
+          Row<T>::unpack(d, now.ds.raw[v]);
 #pragma unroll
-      for (int v = 0; v < NV; ++v) now.x.raw[v] = Row<T>::pack(g[v]);
+          for (int j = 0; j < VE; ++j) g[v][j] = fmaf(now.rstd, g[v][j], d[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < VE; ++j) g[v][j] *= now.rstd;
+        }
+        now.x.raw[v] = Row<T>::pack(g[v]);
+      }
       team.store(now.x.raw, p.dx, p.dx_pitch, row, live);
     }
   }
@@ -601,11 +615,15 @@ template <typename T> int norm_rows(NormParams &p, int out, hipStream_t stream) 
     halves = p.res && starts_in_a_dword(p.res, p.res_pitch);
     for (int k = 0; k < p.P; ++k) halves = halves || starts_in_a_dword(p.in[k], p.in_pitch);
   }
-  const unsigned one = waves_for(need, 1), two = waves_for(need, 2), four = waves_for(need, 4);
+  // One vector a lane where there are few rows and time is a matter of the longest chain; otherwise two or three,
+  // whichever leaves fewer places of the team's waves empty, because a wave takes its time however little it holds
+  // (8191 rows of f16, two / three: 4096 columns 24.0 / 24.4 us, 4099 columns 27.0 / 24.8, to 8 bits in groups of
+  // 128 30.7 / 25.9; one a lane 31.9 and 37.3, four 28.8 and 31.1).
+  const unsigned one = waves_for(need, 1), two = waves_for(need, 2), three = waves_for(need, 3), four = waves_for(need, 4);
   if (one == 1) return launch_norm<T, 1>(p, out, halves, 1, 4, stream);
   if (p.rows <= 512 && one <= kMaxWaves) return launch_norm<T, 1>(p, out, halves, one, 1, stream);
-  if (two == 1) return launch_norm<T, 2>(p, out, halves, 1, 4, stream);
-  if (two <= kMaxWaves) return launch_norm<T, 2>(p, out, halves, two, 1, stream);
+  if (3 * three < 2 * two && three <= kMaxWaves) return launch_norm<T, 3>(p, out, halves, three, three == 1 ? 4 : 1, stream);
+  if (two <= kMaxWaves) return launch_norm<T, 2>(p, out, halves, two, two == 1 ? 4 : 1, stream);
   if (four <= kMaxWaves) return launch_norm<T, 4>(p, out, halves, four, 1, stream);
   if constexpr (sizeof(T) == 4) return launch_norm<T, 8>(p, out, halves, waves_for(need, 8), 1, stream);
   return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
