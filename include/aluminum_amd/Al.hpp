@@ -1208,6 +1208,80 @@ void halo_unpack(T *grid, const T *const bufs[6], const size_t dims[3], size_t h
 inline size_t halo_face_elems(const size_t dims[3], size_t halo, int face) {
   return alamd_halo_face_elems(dims, halo, face);
 }
+
+/** Root-mean-square norm of the sum of `ranks` contributions and a residual: what follows the Allreduce of a
+ *  layer's partial results, in the pass that folds them (alamd_rms_norm).  T is a 16-bit float or float, W that or
+ *  float; sum, residual, weight and rstd may be null.  Strides are in elements between rows.  This and the calls
+ *  below run on the communicator's stream; the reference has no counterpart. */
+template <typename T, typename W>
+void rms_norm(T *out, size_t out_stride, T *sum, const T *residual, size_t residual_stride, const T *const *ins, int ranks,
+              size_t in_stride, const W *weight, float *rstd, size_t rows, size_t cols, float eps, Communicator &comm) {
+  std::vector<const void *> tab(ins, ins + (ranks > 0 ? ranks : 0));
+  AL_AMD_CHECK(alamd_rms_norm(out, out_stride, sum, residual, residual_stride, tab.data(), ranks, in_stride, weight,
+                              TypeMap<W>::value, rstd, nullptr, 0, rows, cols, TypeMap<T>::value, eps, comm.get_stream()));
+}
+/** The same to 8 bits an element (e4m3) with a scale for every `group` columns, or for every row (group = 0). */
+template <typename T, typename W>
+void rms_norm_e4m3(uint8_t *out, size_t out_stride, float *scales, size_t group, T *sum, const T *residual, size_t residual_stride,
+                   const T *const *ins, int ranks, size_t in_stride, const W *weight, float *rstd, size_t rows, size_t cols,
+                   float eps, Communicator &comm) {
+  if (!scales) AL_AMD_THROW("An 8-bit output needs scales");
+  std::vector<const void *> tab(ins, ins + (ranks > 0 ? ranks : 0));
+  AL_AMD_CHECK(alamd_rms_norm(out, out_stride, sum, residual, residual_stride, tab.data(), ranks, in_stride, weight,
+                              TypeMap<W>::value, rstd, scales, group, rows, cols, TypeMap<T>::value, eps, comm.get_stream()));
+}
+/** Its backward pass (alamd_rms_norm_grad); `workspace`: rms_norm_grad_workspace(rows, cols) bytes of device memory. */
+inline size_t rms_norm_grad_workspace(size_t rows, size_t cols) { return alamd_rms_norm_grad_workspace(rows, cols); }
+template <typename T, typename W>
+void rms_norm_grad(T *dx, size_t dx_stride, const T *const *dys, int ranks, size_t dy_stride, const T *x, size_t x_stride,
+                   const T *dsum, size_t dsum_stride, const float *rstd, const W *weight, W *dweight, size_t rows, size_t cols,
+                   void *workspace, Communicator &comm) {
+  std::vector<const void *> tab(dys, dys + (ranks > 0 ? ranks : 0));
+  AL_AMD_CHECK(alamd_rms_norm_grad(dx, dx_stride, tab.data(), ranks, dy_stride, x, x_stride, dsum, dsum_stride, rstd, weight,
+                                   TypeMap<W>::value, dweight, rows, cols, TypeMap<T>::value, workspace, comm.get_stream()));
+}
+
+/** A list of buffers, the gradients of a model, with the norm over all of them and the clipping by it
+ *  (alamd_tensor_list).  Belongs to the device that is current when it is made; destroyed when nothing uses it. */
+class TensorList {
+ public:
+  TensorList() = default;
+  TensorList(const TensorList &) = delete;
+  TensorList &operator=(const TensorList &) = delete;
+  ~TensorList() { (void)alamd_tensor_list_destroy(list_); }
+  /** Adds `count` elements at `in`, clipped to `out` or, by default, in place. */
+  template <typename T> void add(T *in, size_t count) { add(in, in, count); }
+  template <typename T> void add(T *out, const T *in, size_t count) {
+    if (list_) AL_AMD_THROW("The tensor list has been made already");
+    outs_.push_back(out);
+    ins_.push_back(in);
+    counts_.push_back(count);
+    dtypes_.push_back(TypeMap<T>::value);
+  }
+  /** Makes the table of what was added; allocates device memory. */
+  void make() {
+    if (list_) AL_AMD_THROW("The tensor list has been made already");
+    AL_AMD_CHECK(alamd_tensor_list_create(&list_, outs_.data(), ins_.data(), counts_.data(), dtypes_.data(), ins_.size()));
+  }
+  /** `norm`: one float in device memory; `workspace`: workspace_bytes of it. */
+  static constexpr size_t workspace_bytes = ALAMD_GLOBAL_NORM_WORKSPACE_BYTES;
+  void global_norm(float *norm, void *workspace, Communicator &comm) const {
+    AL_AMD_CHECK(alamd_global_norm(list_, norm, workspace, comm.get_stream()));
+  }
+  void clip_to_norm(const float *norm, float max_norm, float eps, Communicator &comm) const {
+    AL_AMD_CHECK(alamd_clip_to_norm(list_, norm, max_norm, eps, comm.get_stream()));
+  }
+  void clip_global_norm(float *norm, float max_norm, float eps, void *workspace, Communicator &comm) const {
+    AL_AMD_CHECK(alamd_clip_global_norm(list_, norm, max_norm, eps, workspace, comm.get_stream()));
+  }
+
+ private:
+  std::vector<void *> outs_;
+  std::vector<const void *> ins_;
+  std::vector<size_t> counts_;
+  std::vector<int> dtypes_;
+  alamd_tensor_list *list_ = nullptr;
+};
 }  // namespace amd
 
 /** Host-only completion test; resets the request when complete
