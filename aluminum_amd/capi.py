@@ -358,27 +358,35 @@ def copy(dst, src, nbytes=None, stream=None):
                              _stream(stream)))
 
 
-_TYPE_CODES = {}
+# The operators below are called for single tokens too, where the time of a call is the host's: they look at every
+# tensor once (some 50 ns for each attribute), and ask torch for its module, the device and the stream once a call.
+_torch = None
+_TYPE_CODES = {}  # library number of a torch dtype that rows may have
 
 
-def _type_code(dtype):
-    """Library number of a torch dtype that rows of the operators below may have; None for others."""
-    if not _TYPE_CODES:
-        import torch
-        _TYPE_CODES.update({torch.float16: DTYPES.index("f16"), torch.bfloat16: DTYPES.index("bf16"),
-                            torch.float32: DTYPES.index("f32")})
-    return _TYPE_CODES.get(dtype)
+def _load_torch():
+    global _torch
+    import torch
+    _TYPE_CODES.update({torch.float16: DTYPES.index("f16"), torch.bfloat16: DTYPES.index("bf16"),
+                        torch.float32: DTYPES.index("f32")})
+    _torch = torch
+    return torch
 
 
 def _device_of(t):
     """The device of a tensor, which has to be the current one."""
-    import torch
     dev = t.get_device()
     if dev < 0:
         raise AlError(1, "buffers must live on the GPU")
-    if dev != torch.cuda.current_device():
-        raise AlError(1, "a buffer lives on device %d, the current device is %d" % (dev, torch.cuda.current_device()))
+    now = (_torch or _load_torch()).cuda.current_device()
+    if dev != now:
+        raise AlError(1, "a buffer lives on device %d, the current device is %d" % (dev, now))
     return dev
+
+
+def _stream_on(stream, dev):
+    """_stream for a caller that knows the current device."""
+    return _torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)
 
 
 def _same_device(t, dev):
@@ -387,8 +395,9 @@ def _same_device(t, dev):
                       "a buffer lives on device %d, another one on device %d" % (t.get_device(), dev))
 
 
-def _matrix(t, shape, dtype, dev, what):
-    """(address, elements between rows) of a matrix on the GPU whose rows are contiguous."""
+def _matrix(t, like, dev, dtype, what):
+    """(address, elements between rows) of a matrix on the GPU of like's shape whose rows are contiguous."""
+    shape = like.shape
     if t.shape != shape or t.dtype != dtype:
         raise AlError(1, "%s is %s of %s, expected %s of %s" % (what, tuple(t.shape), t.dtype, tuple(shape), dtype))
     if t.get_device() != dev:
@@ -415,60 +424,68 @@ def _vector(t, n, dtype, dev, what):
     return t.data_ptr()
 
 
-def _rank_matrices(tensors, shape, dtype, dev, what):
-    """Table of the ranks' matrices, which share one distance between rows, and that distance."""
-    first, stride = _matrix(tensors[0], shape, dtype, dev, what)
-    like = tensors[0].stride()
-    at = [first]
+def _rank_matrices(tensors, dev, what):
+    """Table of the ranks' matrices, which share one distance between rows, that distance, and the type's number."""
+    x = tensors[0]
+    if x.dim() != 2:
+        raise AlError(1, "%s is a matrix of [rows, cols]" % what)
+    dtype = x.dtype
+    code = _TYPE_CODES.get(dtype)
+    if code is None:
+        raise AlError(3, "a norm takes float16, bfloat16 or float32 rows, not %s" % dtype)
+    first, stride = _matrix(x, x, dev, dtype, what)
+    n = len(tensors)
+    if n == 1:
+        return (C.c_void_p * 1)(first), stride, code
+    shape, like, at = x.shape, x.stride(), [first]
     for t in tensors[1:]:
         if t.shape != shape or t.dtype != dtype or t.get_device() != dev or t.stride() != like:
-            p, s = _matrix(t, shape, dtype, dev, what)
+            p, s = _matrix(t, x, dev, dtype, what)
             if s != stride and shape[0] > 1:
                 raise AlError(1, "%s of every rank must have the same distance between rows" % what)
             at.append(p)
         else:
             at.append(t.data_ptr())
-    return (C.c_void_p * len(at))(*at), stride
+    return (C.c_void_p * n)(*at), stride, code
+
+
+def _weight(weight, cols, dtype, dev):
+    if weight.dtype != dtype and weight.dtype != _torch.float32:
+        raise AlError(3, "the weight has the rows' type or float32, not %s" % weight.dtype)
+    return _vector(weight, cols, weight.dtype, dev, "weight"), _TYPE_CODES[weight.dtype]
 
 
 def rms_norm(out, ins, weight=None, residual=None, sum_out=None, rstd=None, scales=None, group=0, eps=1e-6, stream=None):
     """out = rms norm of ins[0] + .. + ins[P-1] (+ residual), times weight (alamd_rms_norm).  All matrices are
     [rows, cols] with contiguous rows; `sum_out` receives the sum, `rstd` (fp32, [rows]) what rms_norm_grad needs.
     With `scales` (fp32, [rows, groups]) out is torch.float8_e4m3fn in groups of `group` columns (0: a row)."""
-    import torch
+    if not ins:
+        raise AlError(1, "no rank's input")
     x = ins[0]
-    if x.dim() != 2:
-        raise AlError(1, "rms_norm takes matrices of [rows, cols]")
-    shape, dtype, dev = x.shape, x.dtype, _device_of(x)
-    rows, cols = shape
-    code = _type_code(dtype)
-    if code is None:
-        raise AlError(3, "a norm takes float16, bfloat16 or float32 rows, not %s" % dtype)
-    table, in_stride = _rank_matrices(ins, shape, dtype, dev, "a rank's input")
-    out_p, out_stride = _matrix(out, shape, dtype if scales is None else torch.float8_e4m3fn, dev, "out")
-    res_p = sum_p = None
-    res_stride = 0
+    dev = _device_of(x)
+    table, in_stride, code = _rank_matrices(ins, dev, "a rank's input")
+    dtype = x.dtype
+    rows, cols = x.shape
+    out_p, out_stride = _matrix(out, x, dev, dtype if scales is None else _torch.float8_e4m3fn, "out")
+    res_p = sum_p = rstd_p = scales_p = w_p = None
+    w_code, res_stride = code, 0
     if residual is not None:
-        res_p, res_stride = _matrix(residual, shape, dtype, dev, "residual")
+        res_p, res_stride = _matrix(residual, x, dev, dtype, "residual")
     if sum_out is not None:
-        sum_p, s = _matrix(sum_out, shape, dtype, dev, "sum_out")
+        sum_p, s = _matrix(sum_out, x, dev, dtype, "sum_out")
         if residual is not None and s != res_stride and rows > 1:
             raise AlError(1, "residual and sum_out must have the same distance between rows")
         res_stride = s
-    w_p, w_dt = (None, code) if weight is None else _weight(weight, cols, dtype, dev)
-    groups = -(-cols // group) if group > 0 else 1
-    _check(load().alamd_rms_norm(
-        out_p, out_stride, sum_p, res_p, res_stride, table, len(ins), in_stride, w_p, w_dt,
-        None if rstd is None else _vector(rstd, rows, torch.float32, dev, "rstd"),
-        None if scales is None else _vector(scales, rows * groups, torch.float32, dev, "scales"),
-        group, rows, cols, code, eps, _stream(stream)))
-
-
-def _weight(weight, cols, dtype, dev):
-    import torch
-    if weight.dtype != dtype and weight.dtype != torch.float32:
-        raise AlError(3, "the weight has the rows' type or float32, not %s" % weight.dtype)
-    return _vector(weight, cols, weight.dtype, dev, "weight"), _type_code(weight.dtype)
+    if weight is not None:
+        w_p, w_code = _weight(weight, cols, dtype, dev)
+    if rstd is not None:
+        rstd_p = _vector(rstd, rows, _torch.float32, dev, "rstd")
+    if scales is not None:
+        scales_p = _vector(scales, rows * (-(-cols // group) if group > 0 else 1), _torch.float32, dev, "scales")
+    rc = load().alamd_rms_norm(out_p, out_stride, sum_p, res_p, res_stride, table, len(ins), in_stride, w_p, w_code, rstd_p,
+                               scales_p, group, rows, cols, code, eps, _stream_on(stream, dev))
+    if rc:
+        _check(rc)
 
 
 def rms_norm_grad_workspace(rows, cols):
@@ -480,34 +497,38 @@ def rms_norm_grad(dx, dys, x, rstd, weight=None, dsum=None, dweight=None, worksp
     """Backward pass of rms_norm (alamd_rms_norm_grad): dx (may be None) from the ranks' gradients dys of the
     output and dsum of the sum; dweight (may be None) has the weight's type, or without a weight any that a weight
     may have.  `workspace`: a contiguous tensor of at least rms_norm_grad_workspace(rows, cols) bytes."""
-    import torch
-    if x.dim() != 2:
-        raise AlError(1, "rms_norm_grad takes matrices of [rows, cols]")
-    shape, dtype, dev = x.shape, x.dtype, _device_of(x)
-    rows, cols = shape
-    code = _type_code(dtype)
-    if code is None:
-        raise AlError(3, "a norm takes float16, bfloat16 or float32 rows, not %s" % dtype)
-    table, dy_stride = _rank_matrices(dys, shape, dtype, dev, "a rank's gradient")
-    x_p, x_stride = _matrix(x, shape, dtype, dev, "x")
-    dx_p, dx_stride = (None, cols) if dx is None else _matrix(dx, shape, dtype, dev, "dx")
-    ds_p, ds_stride = (None, cols) if dsum is None else _matrix(dsum, shape, dtype, dev, "dsum")
-    w_p, w_dt = (None, code) if weight is None else _weight(weight, cols, dtype, dev)
-    dw_p = ws_p = None
+    if not dys:
+        raise AlError(1, "no rank's gradient")
+    dev = _device_of(x)
+    table, dy_stride, code = _rank_matrices(dys, dev, "a rank's gradient")
+    dtype = dys[0].dtype
+    x_p, x_stride = _matrix(x, dys[0], dev, dtype, "x")
+    rows, cols = x.shape
+    dx_p = ds_p = w_p = dw_p = ws_p = None
+    dx_stride = ds_stride = cols
+    w_code = code
+    if dx is not None:
+        dx_p, dx_stride = _matrix(dx, x, dev, dtype, "dx")
+    if dsum is not None:
+        ds_p, ds_stride = _matrix(dsum, x, dev, dtype, "dsum")
+    if weight is not None:
+        w_p, w_code = _weight(weight, cols, dtype, dev)
     if dweight is not None:
         if weight is None:
-            dw_p, w_dt = _weight(dweight, cols, dtype, dev)
+            dw_p, w_code = _weight(dweight, cols, dtype, dev)
         else:
             dw_p = _vector(dweight, cols, weight.dtype, dev, "dweight")
         if rows:
-            need = rms_norm_grad_workspace(rows, cols)
+            need = load().alamd_rms_norm_grad_workspace(rows, cols)
             have = 0 if workspace is None else workspace.numel() * workspace.element_size()
             if have < need:
                 raise AlError(1, "dweight needs a workspace of %d bytes, not %d" % (need, have))
             ws_p = _vector(workspace, workspace.numel(), workspace.dtype, dev, "workspace")
-    _check(load().alamd_rms_norm_grad(
-        dx_p, dx_stride, table, len(dys), dy_stride, x_p, x_stride, ds_p, ds_stride,
-        _vector(rstd, rows, torch.float32, dev, "rstd"), w_p, w_dt, dw_p, rows, cols, code, ws_p, _stream(stream)))
+    rc = load().alamd_rms_norm_grad(dx_p, dx_stride, table, len(dys), dy_stride, x_p, x_stride, ds_p, ds_stride,
+                                    _vector(rstd, rows, _torch.float32, dev, "rstd"), w_p, w_code, dw_p, rows, cols, code,
+                                    ws_p, _stream_on(stream, dev))
+    if rc:
+        _check(rc)
 
 
 class TensorList:
@@ -518,7 +539,7 @@ class TensorList:
     WORKSPACE_BYTES = 16384
 
     def __init__(self, ins, outs=None):
-        import torch
+        torch = _torch or _load_torch()
         self._h = C.c_void_p(None)
         self._keep = (list(ins), None if outs is None else list(outs))
         n = len(self._keep[0])
@@ -545,8 +566,7 @@ class TensorList:
         return _vector(workspace, workspace.numel(), workspace.dtype, self._dev, "workspace")
 
     def _norm(self, norm):
-        import torch
-        return _vector(norm, 1, torch.float32, self._dev, "norm")
+        return _vector(norm, 1, _torch.float32, self._dev, "norm")
 
     def global_norm(self, norm, workspace=None, stream=None):
         """norm[0] = the norm over all elements (alamd_global_norm)."""

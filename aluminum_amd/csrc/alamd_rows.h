@@ -312,6 +312,11 @@ template <typename T, int NV, bool HALVES> struct RowTeam {
       else __builtin_amdgcn_raw_buffer_store_b32(d[0], r, at, 0, kAuxStoreRow);
     }
   }
+  // x as a vector of a row that is the team's alone.
+  __device__ __forceinline__ void store_vector(const float (&x)[VE], int v, char *base) const {
+    const auto r = rsrc(base, 0, 0, true, cols * (unsigned)sizeof(T));
+    __builtin_amdgcn_raw_buffer_store_b128(Row<T>::pack(x), r, off[v], 0, 0);
+  }
   // x to elements of an fp32 row.
   __device__ __forceinline__ void store_f32(const float (&x)[VE], int v, float *row) const {
     if (off[v] == kNowhere) return;

@@ -249,6 +249,8 @@ struct GradParams {
   char *dx;
   const float *rstd;
   float *partial;  // [workgroups][cols]: the weight's gradient from each workgroup's rows
+  char *dweight;   // where a launch of one workgroup writes it to
+  int dw32;        // in fp32
   unsigned long long dy_pitch, x_pitch, dsum_pitch, dx_pitch;
   unsigned long long rows;
   unsigned cols;
@@ -383,6 +385,11 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
   }
   if (!p.partial) return;
   float *dst = p.partial + (size_t)blockIdx.x * p.cols;
+  auto put = [&](const float (&d)[VE], int v) {
+    if (gridDim.x > 1) team.store_f32(d, v, dst);
+    else if (p.dw32) team.store_f32(d, v, reinterpret_cast<float *>(p.dweight));
+    else team.store_vector(d, v, p.dweight);
+  };
   if constexpr (WIDE) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
         const float4 a = slot(v, j);
         d[j] = a.x, d[j + 1] = a.y, d[j + 2] = a.z, d[j + 3] = a.w;
       }
-      team.store_f32(d, v, dst);
+      put(d, v);
     }
   } else {
     // the upper half of the teams hands its part to the lower half, until one team has all
@@ -423,7 +430,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
     }
     if (team.index == 0) {
 #pragma unroll
-      for (int v = 0; v < NV; ++v) team.store_f32(dw[v], v, dst);
+      for (int v = 0; v < NV; ++v) put(dw[v], v);
     }
   }
 }
@@ -637,7 +644,8 @@ int launch_grad_b(GradParams &p, size_t *parts, unsigned waves, unsigned teams, 
   p.shape = {waves, teams};
   size_t grid = (p.rows + teams - 1) / teams;
   if (grid > kGradParts) grid = kGradParts;
-  *parts = grid;
+  if (p.partial && p.rows <= 2 * (size_t)teams) grid = 1;
+  *parts = grid == 1 ? 0 : grid;  // one workgroup has written the weight's gradient itself
   const size_t lds = (WIDE ? 1 : teams / 2) * (size_t)waves * 64 * NV * Row<T>::VE * sizeof(float);
   hipLaunchKernelGGL((rms_norm_grad_kernel<T, NV, B, WIDE, THREADS>), dim3((unsigned)grid), dim3(64 * waves * teams), lds, stream, p);
   ALAMD_HIP(hipGetLastError());
@@ -645,8 +653,12 @@ int launch_grad_b(GradParams &p, size_t *parts, unsigned waves, unsigned teams, 
 }
 template <typename T, int NV, int THREADS>
 int launch_grad(GradParams &p, size_t *parts, unsigned waves, hipStream_t stream) {
+  // As many rows a workgroup as it has waves for, so that there are few parts to join; but every CU gets a row first,
+  // except where one workgroup does the whole call in two turns, which saves the second launch.
   unsigned teams = THREADS / 64 / waves;
-  while (teams > 1 && p.rows < (size_t)256 * teams) --teams;
+  if (!p.partial || p.rows > 2 * (size_t)teams)
+    while (teams > 1 && p.rows < (size_t)256 * teams) --teams;
+  if (teams > p.rows) teams = (unsigned)p.rows;
   return p.P == 1 ? launch_grad_b<T, NV, 1, false, THREADS>(p, parts, waves, teams, stream)
                   : launch_grad_b<T, NV, 4, false, THREADS>(p, parts, waves, teams, stream);
 }
@@ -789,6 +801,8 @@ int alamd_rms_norm_grad(void *dx, size_t dx_stride, const void *const *dys, int 
     p.dx = static_cast<char *>(dx);
     p.rstd = rstd;
     p.partial = dweight ? static_cast<float *>(workspace) : nullptr;
+    p.dweight = static_cast<char *>(dweight);
+    p.dw32 = weight_dtype == ALAMD_F32;
     p.dy_pitch = dy_stride * es;
     p.x_pitch = x_stride * es;
     p.dsum_pitch = dsum_stride * es;
@@ -808,7 +822,7 @@ int alamd_rms_norm_grad(void *dx, size_t dx_stride, const void *const *dys, int 
     }
     if (rc) return rc;
   }
-  if (!dweight) return ALAMD_OK;
+  if (!dweight || (rows > 0 && parts == 0)) return ALAMD_OK;
   const dim3 grid((unsigned)((cols + 31) / 32));
   const float *partial = static_cast<const float *>(workspace);
   switch (weight_dtype) {
