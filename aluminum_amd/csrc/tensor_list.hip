@@ -233,9 +233,12 @@ int launch_clip(const alamd_tensor_list *list, bool cached, const double *parts,
   return ALAMD_OK;
 }
 
-int check_workspace(const void *workspace) {
+int check_workspace(const void *workspace, const float *norm) {
   if (!workspace || !aligned_to(workspace, 8))
     return set_error(ALAMD_ERR_INVALID_ARG, "the workspace is null or not aligned to 8 bytes");
+  const uintptr_t w = reinterpret_cast<uintptr_t>(workspace), n = reinterpret_cast<uintptr_t>(norm);
+  if (n + sizeof(float) > w && n < w + ALAMD_GLOBAL_NORM_WORKSPACE_BYTES)
+    return set_error(ALAMD_ERR_OVERLAP, "the norm lies in the workspace");
   return ALAMD_OK;
 }
 
@@ -325,7 +328,7 @@ int alamd_tensor_list_destroy(alamd_tensor_list *list) {
 int alamd_global_norm(const alamd_tensor_list *list, float *norm, void *workspace, void *stream) {
   if (int rc = check_list(list)) return rc;
   if (int rc = check_clip(norm, 0.0f, 0.0f)) return rc;
-  if (int rc = check_workspace(workspace)) return rc;
+  if (int rc = check_workspace(workspace, norm)) return rc;
   return launch_norm(list, norm, static_cast<double *>(workspace), as_stream(stream));
 }
 
@@ -339,7 +342,7 @@ int alamd_clip_global_norm(const alamd_tensor_list *list, float *norm, float max
                            void *stream) {
   if (int rc = check_list(list)) return rc;
   if (int rc = check_clip(norm, max_norm, eps)) return rc;
-  if (int rc = check_workspace(workspace)) return rc;
+  if (int rc = check_workspace(workspace, norm)) return rc;
   double *parts = static_cast<double *>(workspace);
   if (list->chunks == 0) return launch_norm(list, norm, parts, as_stream(stream));
   const bool cached = list->bytes <= kCachedBytes;

@@ -438,8 +438,11 @@ int alamd_copy(void *dst, const void *src, size_t bytes, void *stream);
  * `sum` and `out` may each take the place of an input or of the residual (the
  * same address and stride, and for `out` no scales); other overlaps are
  * ALAMD_ERR_OVERLAP.  cols is at most ALAMD_RMS_NORM_MAX_COLS.  Nothing is done
- * for rows = 0 or cols = 0.  A result depends on the values alone, not on the
- * stream, the rows around it or the run. */
+ * for rows = 0 or cols = 0.  A row whose squares overflow fp32 has rstd = 0.
+ * The order of the additions depends on rows, cols, P and the types alone: the
+ * same call gives the same bits every time.  (A row of 16-bit elements that
+ * starts in the middle of a dword is read together with the two bytes in front
+ * of it, which share that dword.) */
 #define ALAMD_RMS_NORM_MAX_COLS 32768
 int alamd_rms_norm(void *out, size_t out_stride, void *sum, const void *residual,
                    size_t residual_stride, const void *const *ins, int P, size_t in_stride,
@@ -488,7 +491,8 @@ int alamd_tensor_list_destroy(alamd_tensor_list *list);
 /* *norm (fp32, device memory) = sqrt of the sum of the squares of every element
  * of the list, squared and summed in fp64 in an order that depends on the list
  * alone; 0 for an empty list.  `workspace`: ALAMD_GLOBAL_NORM_WORKSPACE_BYTES of
- * device memory, aligned to 8 bytes, that no call running at the same time uses. */
+ * device memory, aligned to 8 bytes, that no call running at the same time uses.
+ * Neither it nor the norm is part of the list or of the other. */
 #define ALAMD_GLOBAL_NORM_WORKSPACE_BYTES 16384
 int alamd_global_norm(const alamd_tensor_list *list, float *norm, void *workspace, void *stream);
 

@@ -449,3 +449,71 @@ def test_captured_and_on_another_stream(al):
         side.synchronize()
         for a, b in zip(results(), want):
             assert torch.equal(a, b)
+
+
+def test_refusals(al):
+    """What the binding and the library refuse, with nothing written."""
+    import torch
+    x, y = torch.ones(6, 64, device="cuda"), torch.full((6, 64), 7.0, device="cuda")
+    wide = torch.ones(6, 128, device="cuda")
+    rstd, w = torch.ones(6, device="cuda"), torch.ones(64, device="cuda")
+    q, sc = torch.zeros(6, 64, dtype=torch.float8_e4m3fn, device="cuda"), torch.ones(6, 2, device="cuda")
+    dw = torch.full((64,), 7.0, device="cuda")
+    ws = torch.empty(al.rms_norm_grad_workspace(6, 64), dtype=torch.uint8, device="cuda")
+    for code, call in [
+            (1, lambda: al.rms_norm(y, [])), (1, lambda: al.rms_norm(y, [x[0]])), (1, lambda: al.rms_norm(y[:5], [x])),
+            (1, lambda: al.rms_norm(y.bfloat16(), [x])), (1, lambda: al.rms_norm(y, [x, x.bfloat16()])),
+            (1, lambda: al.rms_norm(y, [x, wide[:, :64]])), (1, lambda: al.rms_norm(y, [x, x[:, :63]])),
+            (1, lambda: al.rms_norm(y, [x.cpu()])), (1, lambda: al.rms_norm(y, [x, x.cpu()])), (1, lambda: al.rms_norm(y, [wide[:, ::2]])),
+            (1, lambda: al.rms_norm(y, [x[:1].expand(6, 64)])), (3, lambda: al.rms_norm(y.double(), [x.double()])),
+            (1, lambda: al.rms_norm(y, [x], weight=w[:63])), (3, lambda: al.rms_norm(y, [x], weight=w.half())),
+            (1, lambda: al.rms_norm(y, [x], residual=x, sum_out=wide[:, :64])), (1, lambda: al.rms_norm(y, [x], rstd=rstd[:5])),
+            (1, lambda: al.rms_norm(y, [x], rstd=rstd.double())), (1, lambda: al.rms_norm(y, [x], scales=sc, group=32)),
+            (1, lambda: al.rms_norm(q, [x], scales=sc, group=48)), (1, lambda: al.rms_norm(q, [x], scales=sc)),
+            (1, lambda: al.rms_norm(q, [x])), (1, lambda: al.rms_norm(y, [x], group=32)), (1, lambda: al.rms_norm(y, [x], eps=-1.0)),
+            (5, lambda: al.rms_norm(wide[:, 1:65], [wide[:, :64]])), (5, lambda: al.rms_norm(y, [x], residual=x, sum_out=y)),
+            (1, lambda: al.rms_norm_grad(y, [], x, rstd)), (1, lambda: al.rms_norm_grad(None, [x], x, rstd)),
+            (1, lambda: al.rms_norm_grad(y, [x], x.half(), rstd)), (1, lambda: al.rms_norm_grad(y, [x], x, rstd[:5])),
+            (1, lambda: al.rms_norm_grad(y, [x], x, rstd, dweight=dw)), (1, lambda: al.rms_norm_grad(y, [x], x, rstd, dweight=dw, workspace=ws[:-1])),
+            (1, lambda: al.rms_norm_grad(y, [x], x, rstd, weight=w, dweight=dw.half(), workspace=ws)),
+            (1, lambda: al.rms_norm_grad(None, [x], x, rstd, dsum=x, dweight=dw, workspace=ws)),
+            (5, lambda: al.rms_norm_grad(wide[:, 1:65], [x], wide[:, :64], rstd)),
+            (5, lambda: al.rms_norm_grad(y, [x], x, rstd, weight=w, dweight=ws.view(torch.float32)[:64], workspace=ws))]:
+        with pytest.raises(al.AlError) as e:
+            call()
+        assert e.value.code == code, e.value
+    torch.cuda.synchronize()
+    assert bool((y == 7).all()) and bool((dw == 7).all()) and bool((x == 1).all()) and bool((wide == 1).all())
+
+
+def test_two_streams_at_once(al):
+    """Calls on two streams at once, each with its own buffers."""
+    import torch
+    side = [torch.cuda.Stream() for _ in range(2)]
+    sets = []
+    for k in range(2):
+        gen = torch.Generator(device="cuda").manual_seed(k)
+        x, t = (torch.randn(3000, 1537, device="cuda", generator=gen).bfloat16() for _ in range(2))
+        w = torch.rand(1537, device="cuda", generator=gen)
+        ws = torch.empty(al.rms_norm_grad_workspace(3000, 1537), dtype=torch.uint8, device="cuda")
+        sets.append((x, t, w, ws, torch.empty_like(x), torch.empty_like(x), torch.empty(3000, device="cuda"), torch.empty_like(w)))
+
+    def both(s, stream):
+        x, t, w, ws, out, dx, rstd, dw = s
+        al.rms_norm(out, [x, t], weight=w, rstd=rstd, stream=stream)
+        al.rms_norm_grad(dx, [t], x, rstd, weight=w, dweight=dw, workspace=ws, stream=stream)
+
+    want = []
+    for s in sets:
+        both(s, None)
+        torch.cuda.synchronize()
+        want.append([v.clone() for v in s[4:]])
+        for v in s[4:]:
+            v.zero_()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, stream in zip(sets, side):
+            both(s, stream)
+    torch.cuda.synchronize()
+    for s, w in zip(sets, want):
+        assert all(torch.equal(a, b) for a, b in zip(s[4:], w))

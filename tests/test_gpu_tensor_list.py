@@ -229,6 +229,37 @@ def test_captured_and_on_another_stream(al):
             assert all(torch.equal(a, b) for a, b in zip(w, outs + [norm]))
 
 
+def test_refusals(al):
+    import torch
+    t = [torch.ones(100, device="cuda"), torch.ones(100, device="cuda").half()]
+    lst = al.TensorList(t)
+    norm = torch.zeros(1, device="cuda")
+    space = torch.zeros(al.TensorList.WORKSPACE_BYTES + 64, dtype=torch.uint8, device="cuda")
+    for code, call in [
+            (1, lambda: lst.global_norm(torch.zeros(2, device="cuda"))), (1, lambda: lst.global_norm(norm.double())),
+            (1, lambda: lst.global_norm(norm.cpu())), (1, lambda: lst.global_norm(norm, workspace=space[:100])),
+            (1, lambda: lst.global_norm(norm, workspace=space[4:])),
+            (5, lambda: lst.global_norm(space.view(torch.float32)[4:5], workspace=space)),
+            (5, lambda: lst.clip_global_norm(space.view(torch.float32)[-17:-16], 1.0, workspace=space)),
+            (1, lambda: lst.clip_to_norm(norm, -1.0)), (1, lambda: lst.clip_to_norm(norm, float("nan"))),
+            (1, lambda: lst.clip_global_norm(norm, 1.0, eps=-1e-6)), (1, lambda: lst.clip_global_norm(norm, 1.0, eps=float("nan"))),
+            (5, lambda: al.TensorList([t[0], t[0]])), (5, lambda: al.TensorList([t[0], t[0][50:]])),
+            (5, lambda: al.TensorList([t[0][:50]], [t[0][20:70]])),
+            (1, lambda: al.TensorList(t, t[:1])), (1, lambda: al.TensorList(t, [t[1], t[0]])),
+            (1, lambda: al.TensorList([torch.ones(8, 8, device="cuda").t()[1:]])),
+            (3, lambda: al.TensorList([torch.ones(8, device="cuda", dtype=torch.int32)])),
+            (3, lambda: al.TensorList([torch.ones(8, device="cuda", dtype=torch.float64)]))]:
+        with pytest.raises(al.AlError) as e:
+            call()
+        assert e.value.code == code, e.value
+    lst.destroy()
+    lst.destroy()
+    with pytest.raises(al.AlError):
+        lst.global_norm(norm)
+    torch.cuda.synchronize()
+    assert all(bool((v == 1).all()) for v in t)
+
+
 def test_a_training_step(al):
     """Two data-parallel ranks, each with a layer split over three: the norm over the three partial sums, its backward
     pass, the average of the two ranks' gradients, their norm and the clipping; against differentiation of the same
