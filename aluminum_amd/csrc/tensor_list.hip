@@ -41,10 +41,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kU = 4;  // vectors a lane has under way (2 or 8: up to 3 % slower)
 constexpr size_t kChunkBytes = (size_t)64 << 10;
-// Norm and clipping in one call read a list of up to this size through the caches, whose memory-side 256 MiB then hold
-// most of it for the second pass; a longer one past them (us, through / past: lists of 30 MiB 17.9 / 21.7, 207 MiB
-// 108 / 117, 272 MiB 140 / 150, 1.3 GiB 747 / 687; keeping the last 64 to 224 MiB of that: 682 to 708).
-constexpr size_t kCachedBytes = (size_t)288 << 20;
 constexpr size_t kParts = ALAMD_GLOBAL_NORM_WORKSPACE_BYTES / sizeof(double);
 
 // ---- norm -------------------------------------------------------------------
@@ -131,38 +127,48 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double *parts, uns
 
 // ---- clipping ---------------------------------------------------------------
 
-template <typename T, int AUX> __device__ __forceinline__ void chunk_scale(const Chunk &c, float by) {
+// A chunk's part that `LANES` lanes with U vectors each take, from vector `from` on; with it the chunk's elements
+// outside of its vectors where `ends` is set.
+template <typename T, int LANES, int U, int AUX>
+__device__ __forceinline__ void scale_part(const Chunk &c, float by, unsigned from, unsigned step, bool ends) {
   constexpr unsigned VE = Row<T>::VE;
   const unsigned head = (unsigned)head_count(sizeof(T), c.out, c.in, c.count), vecs = (c.count - head) / VE;
   const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(c.in + head * sizeof(T)), 0, (int)(vecs * 16u), kRsrcFlags);
   const auto w = __builtin_amdgcn_make_buffer_rsrc(c.out + head * sizeof(T), 0, (int)(vecs * 16u), kRsrcFlags);
-  for (unsigned i = threadIdx.x; i < vecs + threadIdx.x; i += kThreads * kU) {
-    u32x4 raw[kU];
+  for (unsigned i = from; i < vecs; i += step) {
+    u32x4 raw[U];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) raw[u] = __builtin_amdgcn_raw_buffer_load_b128(r, (i + (unsigned)u * kThreads) * 16u, 0, AUX);
+    for (int u = 0; u < U; ++u) raw[u] = __builtin_amdgcn_raw_buffer_load_b128(r, (i + threadIdx.x + (unsigned)u * LANES) * 16u, 0, AUX);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < U; ++u) {
       float x[VE];
       Row<T>::unpack(x, raw[u]);
 #pragma unroll
       for (unsigned j = 0; j < VE; ++j) x[j] *= by;
-      __builtin_amdgcn_raw_buffer_store_b128(Row<T>::pack(x), w, (i + (unsigned)u * kThreads) * 16u, 0, kAuxStoreRow);
+      __builtin_amdgcn_raw_buffer_store_b128(Row<T>::pack(x), w, (i + threadIdx.x + (unsigned)u * LANES) * 16u, 0, kAuxStoreRow);
     }
   }
+  if (!ends) return;
   if (threadIdx.x < head) Row<T>::put(c.out, threadIdx.x, Row<T>::get(c.in, threadIdx.x) * by);
   const unsigned e = head + vecs * VE + threadIdx.x;
   if (e < c.count) Row<T>::put(c.out, e, Row<T>::get(c.in, e) * by);
 }
-
-template <int AUX> __device__ __forceinline__ void chunk_scale(const Chunk &c, float by) {
-  if (c.dtype == ALAMD_F32) chunk_scale<float, AUX>(c, by);
-  else if (c.dtype == ALAMD_BF16) chunk_scale<bf16_t, AUX>(c, by);
-  else chunk_scale<f16_t, AUX>(c, by);
+template <int LANES, int U, int AUX>
+__device__ __forceinline__ void scale_part(const Chunk &c, float by, unsigned from, unsigned step, bool ends) {
+  if (c.dtype == ALAMD_F32) scale_part<float, LANES, U, AUX>(c, by, from, step, ends);
+  else if (c.dtype == ALAMD_BF16) scale_part<bf16_t, LANES, U, AUX>(c, by, from, step, ends);
+  else scale_part<f16_t, LANES, U, AUX>(c, by, from, step, ends);
 }
 
-// Clips to the norm in *norm, or, with `parts`, to the norm that those make, which the first workgroup writes to
-// *norm.  From the last chunk to the first: what the pass before has read last is the likeliest to be in a cache.
-template <bool PARTS, int AUX>
+__device__ __forceinline__ float clip_factor(float norm, float max_norm, float eps) {
+  norm += eps;
+  return norm <= max_norm ? 1.0f : max_norm / norm;
+}
+
+// A workgroup a chunk.  Clips to the norm in *norm, or, with PARTS, to the norm that those make, which the first
+// workgroup writes to *norm: a launch less.  From the last chunk to the first: what the pass before has read last
+// is the likeliest to be in a cache.
+template <bool PARTS>
 __global__ void __launch_bounds__(kThreads) clip_kernel(const Chunk *table, unsigned long long chunks, const double *parts, unsigned n,
                                                         float *norm, float max_norm, float eps) {
   Chunk next = table[chunks - 1 - blockIdx.x];
@@ -173,14 +179,27 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const Chunk *table, unsi
   } else {
     total = *norm;
   }
-  total += eps;
-  const float by = total <= max_norm ? 1.0f : max_norm / total;
+  const float by = clip_factor(total, max_norm, eps);
   for (unsigned long long k = blockIdx.x; k < chunks; k += gridDim.x) {
     const Chunk c = next;
     next = table[k + gridDim.x < chunks ? chunks - 1 - k - gridDim.x : 0];
     if (by == 1.0f && c.in == c.out) continue;  // nothing to clip
-    chunk_scale<AUX>(c, by);
+    scale_part<kThreads, kU, kAuxLoadCached>(c, by, 0, kThreads * kU, true);
   }
+}
+
+// A wave for every KiB: the addresses that are under way at once stay close together, which a long list's pass is
+// faster for (2.75 GB read and written after the norm: 407 us, with a chunk of 64 KiB a workgroup 460 us, with 16 KiB
+// 450 us; fewer waves a CU than fit, as the folds like it, cost 5 to 15 %).
+constexpr unsigned kTile = 64, kTilesPerChunk = kChunkBytes / 16 / kTile;
+template <int AUX>
+__global__ void __launch_bounds__(kTile) clip_tile_kernel(const Chunk *table, const float *norm, float max_norm, float eps) {
+  // the last chunk first, as above (table: that chunk)
+  const Chunk c = table[-(ptrdiff_t)(blockIdx.x / kTilesPerChunk)];
+  const unsigned tile = blockIdx.x % kTilesPerChunk;
+  const float by = clip_factor(*norm, max_norm, eps);
+  if (by == 1.0f && c.in == c.out) return;
+  scale_part<kTile, 1, AUX>(c, by, tile * kTile, kTilesPerChunk * kTile, tile == 0);  // one turn
 }
 
 // ---- host side ----------------------------------------------------------------
@@ -203,8 +222,8 @@ int check_clip(const float *norm, float max_norm, float eps) {
 }
 
 // Workgroups of a pass; one that has done its chunk takes the next one that far on.  The norm runs at the rate of a large
-// copy with four or two workgroups a CU (847 MB of bf16: 130 us, 6.5 TB/s; eight a CU 136 us); the clipping likes one
-// chunk a workgroup (2.8 GB read and written after the norm: 687 us; 2048 workgroups 718 us).
+// copy with four or two workgroups a CU (847 MB of bf16: 130 us, 6.5 TB/s; eight a CU 136 us); the clipping by chunks
+// likes one of them a workgroup.
 constexpr size_t kNormGrid = 1024, kClipGrid = (size_t)1 << 16;
 static_assert(kNormGrid <= kParts, "the workspace holds a part of every workgroup");
 
@@ -216,19 +235,38 @@ unsigned launch_squares(const alamd_tensor_list *list, bool cached, double *part
   return grid;
 }
 
-int launch_norm(const alamd_tensor_list *list, float *norm, double *parts, hipStream_t stream) {
-  const unsigned n = launch_squares(list, false, parts, stream);
+int launch_norm(const alamd_tensor_list *list, bool cached, float *norm, double *parts, hipStream_t stream) {
+  const unsigned n = launch_squares(list, cached, parts, stream);
   hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, stream, parts, n, norm);
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
 
+// Norm and clipping in one call read a list of up to kCachedBytes through the caches, whose memory-side 256 MiB then
+// hold most of it for the second pass; a longer one past them (us, through / past: lists of 30 MiB 17.9 / 21.7,
+// 207 MiB 108 / 117, 272 MiB 140 / 150, 1.3 GiB 747 / 687; keeping the last 64 to 224 MiB of that: 682 to 708).
+constexpr size_t kCachedBytes = (size_t)288 << 20;
+// From kTiledBytes on a list whose chunks are not small is clipped KiB by KiB, with the norm made in a launch of its own
+// (us, tiles / chunks: 30 MiB 19.2 / 17.8, 114 MiB of long tensors 78.1 / 80.5, 272 MiB 129 / 134, 1.3 GiB 613 / 672).
+constexpr size_t kTiledBytes = (size_t)64 << 20;
+bool in_tiles(const alamd_tensor_list *list) { return list->bytes >= kTiledBytes && list->bytes / list->chunks >= kChunkBytes / 2; }
+
+// Clips to *norm, or by chunks with `parts` to what those make.
 int launch_clip(const alamd_tensor_list *list, bool cached, const double *parts, unsigned n, float *norm, float max_norm, float eps,
                 hipStream_t stream) {
-  const unsigned grid = (unsigned)(list->chunks < kClipGrid ? list->chunks : kClipGrid);
-  auto kern = !parts ? clip_kernel<false, kAuxLoadStream>
-              : cached ? clip_kernel<true, kAuxLoadCached> : clip_kernel<true, kAuxLoadStream>;
-  if (grid) hipLaunchKernelGGL(kern, dim3(grid), dim3(kThreads), 0, stream, list->table, list->chunks, parts, n, norm, max_norm, eps);
+  if (!parts && in_tiles(list)) {
+    constexpr size_t most = (size_t)1 << 18;  // chunks of a launch: 2^24 workgroups
+    auto kern = cached ? clip_tile_kernel<kAuxLoadCached> : clip_tile_kernel<kAuxLoadStream>;
+    for (size_t left = list->chunks; left > 0;) {
+      const size_t now = left < most ? left : most;
+      hipLaunchKernelGGL(kern, dim3((unsigned)now * kTilesPerChunk), dim3(kTile), 0, stream, list->table + left - 1, norm, max_norm, eps);
+      left -= now;
+    }
+  } else if (list->chunks > 0) {
+    const unsigned grid = (unsigned)(list->chunks < kClipGrid ? list->chunks : kClipGrid);
+    hipLaunchKernelGGL(parts ? clip_kernel<true> : clip_kernel<false>, dim3(grid), dim3(kThreads), 0, stream, list->table,
+                       list->chunks, parts, n, norm, max_norm, eps);
+  }
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
@@ -329,7 +367,7 @@ int alamd_global_norm(const alamd_tensor_list *list, float *norm, void *workspac
   if (int rc = check_list(list)) return rc;
   if (int rc = check_clip(norm, 0.0f, 0.0f)) return rc;
   if (int rc = check_workspace(workspace, norm)) return rc;
-  return launch_norm(list, norm, static_cast<double *>(workspace), as_stream(stream));
+  return launch_norm(list, false, norm, static_cast<double *>(workspace), as_stream(stream));
 }
 
 int alamd_clip_to_norm(const alamd_tensor_list *list, const float *norm, float max_norm, float eps, void *stream) {
@@ -344,8 +382,11 @@ int alamd_clip_global_norm(const alamd_tensor_list *list, float *norm, float max
   if (int rc = check_clip(norm, max_norm, eps)) return rc;
   if (int rc = check_workspace(workspace, norm)) return rc;
   double *parts = static_cast<double *>(workspace);
-  if (list->chunks == 0) return launch_norm(list, norm, parts, as_stream(stream));
   const bool cached = list->bytes <= kCachedBytes;
+  if (list->chunks == 0 || in_tiles(list)) {
+    if (int rc = launch_norm(list, cached, norm, parts, as_stream(stream))) return rc;
+    return launch_clip(list, cached, nullptr, 0, norm, max_norm, eps, as_stream(stream));
+  }
   const unsigned n = launch_squares(list, cached, parts, as_stream(stream));
   return launch_clip(list, cached, parts, n, norm, max_norm, eps, as_stream(stream));
 }

@@ -187,6 +187,42 @@ def test_a_tensor_beyond_4_gib(al):
     assert bool((t[-100_000:-1] == 0.25).all())
 
 
+def test_more_chunks_than_one_launch_takes(al):
+    """17 GB in three tensors, of which the first and the last end inside a chunk."""
+    import torch
+    per = CHUNK // 4
+    sizes = [per * 1000 + 5, per * ((1 << 18) + 2) - 7, 3 * per + 1]
+    flat = torch.empty(sum(sizes), device="cuda").fill_(0.5)
+    tensors = list(flat.split(sizes))
+    lst, norm = _call(al, tensors)
+    want = 0.5 * math.sqrt(flat.numel())
+    assert abs(float(norm) - want) <= 1.5 * U32 * want
+    norm.fill_(4.0)
+    lst.clip_to_norm(norm, 1.0, eps=0.0)
+    torch.cuda.synchronize()
+    for t in tensors:
+        assert bool((t == 0.125).all())
+    lst.clip_global_norm(norm, float(norm) + 1e9)  # nothing to clip, and the norm is made anew
+    torch.cuda.synchronize()
+    assert abs(float(norm) - want / 4) <= 1.5 * U32 * want / 4 and bool((tensors[2] == 0.125).all())
+
+
+def test_many_small_tensors(al):
+    """100 MB in tensors of a few KiB: long enough for the clipping by KiB, but of small chunks."""
+    import torch
+    sizes = [2000 + k % 977 for k in range(10_500)]
+    flat = torch.randn(sum(sizes), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    out = torch.empty_like(flat)
+    lst = al.TensorList(list(flat.split(sizes)), list(out.split(sizes)))
+    norm = torch.empty(1, device="cuda")
+    lst.clip_global_norm(norm, 1.0, eps=0.0)
+    torch.cuda.synchronize()
+    want = float(flat.double().square().sum().sqrt())
+    assert abs(float(norm) - want) <= 1.5 * U32 * want
+    w = flat.double() / want
+    assert bool(((out.double() - w).abs() <= 5 * U32 * w.abs() + 2.0 ** -150).all())
+
+
 def test_captured_and_on_another_stream(al):
     """Two lists captured into graphs of their own with a workspace each, replayed with new values and eager work in
     between."""
