@@ -13,10 +13,17 @@
 //   dx = rstd * (g - n_hat * sum(g * n_hat) / n) (+ dsum),   dw = sum over rows of dy * n_hat
 // with the factors of a row gathered: dx = rstd * (g - m * x) + dsum, m = rstd * sum(g * n_hat) / n.
 //
-// A team of TEAM lanes holds a row in registers: NV 128-bit vectors per lane and stream, read once.  The
-// elements behind the last whole vector belong to the next lane, whose vector is moved back so that it ends with
-// the row: its first elements are another lane's as well, computed to the same bits, left out of every sum
-// and stored twice.  Lanes without a vector read zeros and store nothing (the buffer descriptor's bound).
+// A team of waves holds a row in registers: NV 128-bit vectors per lane and stream, read once.  The elements
+// behind the last whole vector belong to the next lane, whose vector is moved back so that it ends with the row:
+// its first elements are another lane's as well, computed to the same bits, left out of every sum and stored
+// twice.  Lanes without a vector read zeros and store nothing (the buffer descriptor's bound).
+//
+// Both passes are bound by memory from a few thousand rows on (8192 x 8192 bf16 with residual and sum: 537 MB in
+// 88 us, 6.1 TB/s, where a large copy reaches 6.5; backward pass of 16384 x 8192 with dsum: 1.07 GB in 178 us,
+// 6.0 TB/s), by the launches and one trip to memory below (one token of 8 x 4096: 3.6 us; backward pass of 64 x
+// 1024 fp32 in two launches 5.1 us), and by their instructions where little moves for an element: with 8-bit
+// outputs (8191 x 4099 f16 in groups of 128: 26 us, of which 16 are the bytes') a wave's fixed part counts, so a
+// row is not cut finer than it has to be and nothing is in a loop that need not be.
 #include "alamd_rows.h"
 
 namespace alamd {
@@ -314,7 +321,8 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
     const bool live = row < p.rows;
     if constexpr (!AHEAD) next.fetch(p, team, row);
     Fetched<T, NV, B> now = next;
-    // the next row's loads are on their way while this one's sum is made and its gradient written
+    // the next row's loads are on their way while this one's sum is made and its gradient written (two or three
+    // rows ahead are no faster: 45.6 and 56.7 us against 43.8 for 4 ranks of 2777 x 5120 f16)
     if constexpr (AHEAD) next.fetch(p, team, row + step);
     float g[NV][VE];
     set_row<T>(g, now.dy[0].raw);
@@ -499,12 +507,15 @@ __global__ void __launch_bounds__(1024) rms_norm_dweight_kernel(char *dw, const 
 
 // ---- host side ----------------------------------------------------------------
 
-// A matrix of the call: a name for messages, the first row, bytes between rows and of a row.
+// A matrix of the call: a name for messages, the first row, bytes between rows and of a row.  A written one may take
+// the place of a read one if both are of the kind that allows it.
+enum Use { READ, READ_REPLACEABLE, WRITTEN, WRITTEN_IN_PLACE };
 struct Matrix {
   const char *name;
   const void *p;
   size_t pitch, bytes;
-  bool written;
+  Use use;
+  bool written() const { return use == WRITTEN || use == WRITTEN_IN_PLACE; }
 };
 
 // Whether two matrices of `rows` rows share memory: by their ranges, or, where rows of the same pitch
@@ -529,13 +540,15 @@ int check_matrix(const void *p, const char *name, size_t stride, size_t rows, si
   return ALAMD_OK;
 }
 
-// Every written matrix against every other one; `same` allows a written matrix to be exactly a read one.
+// Every written matrix against every other one.
 int check_overlaps(const Matrix *m, int n, size_t rows) {
   for (int a = 0; a < n; ++a) {
-    if (!m[a].written || !m[a].p) continue;
+    if (!m[a].written() || !m[a].p) continue;
     for (int b = 0; b < n; ++b) {
-      if (b == a || !m[b].p || (m[b].written && b < a)) continue;
-      if (!m[b].written && m[a].p == m[b].p && (m[a].pitch == m[b].pitch || rows == 1) && m[a].bytes == m[b].bytes) continue;
+      if (b == a || !m[b].p || (m[b].written() && b < a)) continue;
+      if (m[a].use == WRITTEN_IN_PLACE && m[b].use == READ_REPLACEABLE && m[a].p == m[b].p && m[a].bytes == m[b].bytes &&
+          (m[a].pitch == m[b].pitch || rows == 1))
+        continue;
       if (share_memory(m[a], m[b], rows)) return set_error(ALAMD_ERR_OVERLAP, "%s overlaps %s", m[a].name, m[b].name);
     }
   }
@@ -566,7 +579,12 @@ inline bool whole_lines(const void *at, size_t pitch, size_t bytes) {
   return ((reinterpret_cast<uintptr_t>(at) | pitch | bytes) & 63u) == 0;
 }
 
-// A call that moves less than this reads through the caches.
+// A call that moves less than this reads through the caches and stores past them (nt); from there on it reads past
+// them, and writes through where rows cover whole 64-byte pieces.  Both ways in us, bf16 with residual and sum: 134 MB
+// of 4096 x 4096 21.7 / 23.5, 268 MB of 4096 x 8192 48.4 / 47.2, 1.07 GB of 16384 x 8192 188 / 176; read past the
+// caches and written through / nt: 8 ranks of 2048 x 8192 62.5 / 65.3, 16384 rows of 5125 columns, which share their
+// 64-byte pieces, 154 / 126.  The backward pass, which mostly reads, gains from less on (residual's gradient with it,
+// 4096 rows: 34 MB of 1024 columns 11.3 / 11.8, 134 MB of 4096 29.7 / 27.2).
 constexpr size_t kStreamFromBytes = (size_t)256 << 20, kGradStreamFromBytes = (size_t)64 << 20;
 
 // Waves that hold a row of `need` vectors, nv of them a lane.
@@ -622,7 +640,8 @@ template <typename T> int norm_rows(NormParams &p, int out, hipStream_t stream) 
     halves = p.res && starts_in_a_dword(p.res, p.res_pitch);
     for (int k = 0; k < p.P; ++k) halves = halves || starts_in_a_dword(p.in[k], p.in_pitch);
   }
-  // One vector a lane where there are few rows and time is a matter of the longest chain; otherwise two or three,
+  // One vector a lane where there are few rows and time is a matter of the longest chain (one / two in
+  // us: 16 rows of 8192 bf16 3.1 / 3.2; 8191 rows of 5120 f16 33.5 / 29.6); otherwise two or three,
   // whichever leaves fewer places of the team's waves empty, because a wave takes its time however little it holds
   // (8191 rows of f16, two / three: 4096 columns 24.0 / 24.4 us, 4099 columns 27.0 / 24.8, to 8 bits in groups of
   // 128 30.7 / 25.9; one a lane 31.9 and 37.3, four 28.8 and 31.1).
@@ -636,7 +655,9 @@ template <typename T> int norm_rows(NormParams &p, int out, hipStream_t stream) 
   return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
 }
 
-// Workgroups whose partial sums of the weight's gradient are kept.
+// Workgroups whose partial sums of the weight's gradient are kept: one for every CU.  (With two the parts, which grow
+// with them, cost more than the second workgroup gains: 16384 x 8192 bf16 183 us against 179, 4 ranks of 2777 x 5120
+// f16 47.8 against 43.9.)
 constexpr size_t kGradParts = 256;
 
 template <typename T, int NV, int B, bool WIDE, int THREADS>
@@ -675,6 +696,9 @@ template <typename T> int grad_rows(GradParams &p, size_t *parts, hipStream_t st
   }
   const unsigned need = (p.cols + VE - 1) / VE;
   const unsigned one = waves_for(need, 1), two = waves_for(need, 2), four = waves_for(need, 4);
+  // One vector a lane up to 12 waves, two from there on (us, one / two: 256 rows of 4096 bf16 8.1 / 8.6, 4 ranks of 2777 x
+  // 5125 f16 53.7 / 55.7, 16384 x 8192 bf16 182 / 179); rows longer than a workgroup of eight waves can read ahead in its
+  // registers are read as they come.
   if (one <= 12) return launch_grad<T, 1, 1024>(p, parts, one, stream);
   if (two <= 8) return launch_grad<T, 2, 512>(p, parts, two, stream);
   if (two <= kMaxWaves) return launch_grad_b<T, 2, 1, false, 1024>(p, parts, two, 1, stream);
@@ -706,7 +730,7 @@ int alamd_rms_norm(void *out, size_t out_stride, void *sum, const void *residual
   int n = 0, rc;
   for (int k = 0; k < P; ++k) {
     if ((rc = check_matrix(ins[k], "a rank's input", in_stride, rows, cols, es))) return rc;
-    m[n++] = {"a rank's input", ins[k], in_stride * es, cols * es, false};
+    m[n++] = {"a rank's input", ins[k], in_stride * es, cols * es, READ_REPLACEABLE};
   }
   if (residual && (rc = check_matrix(residual, "the residual", residual_stride, rows, cols, es))) return rc;
   if (sum && (rc = check_matrix(sum, "the sum", residual_stride, rows, cols, es))) return rc;
@@ -714,12 +738,12 @@ int alamd_rms_norm(void *out, size_t out_stride, void *sum, const void *residual
   if ((rstd && !aligned_to(rstd, 4)) || (scales && !aligned_to(scales, 4)))
     return set_error(ALAMD_ERR_INVALID_ARG, "rstd or scales not aligned to fp32");
   const size_t groups = scales && group ? (cols + group - 1) / group : 1;
-  m[n++] = {"the residual", residual, residual_stride * es, cols * es, false};
-  m[n++] = {"the weight", weight, 0, cols * wes, false};
-  m[n++] = {"the sum", sum, residual_stride * es, cols * es, true};
-  m[n++] = {"the output", out, out_stride * oes, cols * oes, true};
-  m[n++] = {"rstd", rstd, 4, 4, true};
-  m[n++] = {"the scales", scales, groups * 4, groups * 4, true};
+  m[n++] = {"the residual", residual, residual_stride * es, cols * es, READ_REPLACEABLE};
+  m[n++] = {"the weight", weight, 0, cols * wes, READ};
+  m[n++] = {"the sum", sum, residual_stride * es, cols * es, WRITTEN_IN_PLACE};
+  m[n++] = {"the output", out, out_stride * oes, cols * oes, WRITTEN_IN_PLACE};
+  m[n++] = {"rstd", rstd, 4, 4, WRITTEN};
+  m[n++] = {"the scales", scales, groups * 4, groups * 4, WRITTEN};
   if ((rc = check_overlaps(m, n, rows))) return rc;
   NormParams p{};
   for (int k = 0; k < P; ++k) p.in[k] = static_cast<const char *>(ins[k]);
@@ -773,7 +797,7 @@ int alamd_rms_norm_grad(void *dx, size_t dx_stride, const void *const *dys, int 
     int n = 0, rc;
     for (int k = 0; k < P; ++k) {
       if ((rc = check_matrix(dys[k], "a rank's gradient", dy_stride, rows, cols, es))) return rc;
-      m[n++] = {"a rank's gradient", dys[k], dy_stride * es, cols * es, false};
+      m[n++] = {"a rank's gradient", dys[k], dy_stride * es, cols * es, READ_REPLACEABLE};
     }
     if ((rc = check_matrix(x, "x", x_stride, rows, cols, es))) return rc;
     if (dsum && (rc = check_matrix(dsum, "dsum", dsum_stride, rows, cols, es))) return rc;
@@ -781,16 +805,16 @@ int alamd_rms_norm_grad(void *dx, size_t dx_stride, const void *const *dys, int 
     if (!rstd || !aligned_to(rstd, 4)) return set_error(ALAMD_ERR_INVALID_ARG, "rstd is null or not aligned to fp32");
     if (dweight && (!workspace || !aligned_to(workspace, 4)))
       return set_error(ALAMD_ERR_INVALID_ARG, "dweight needs a workspace aligned to fp32 (alamd_rms_norm_grad_workspace)");
-    m[n++] = {"x", x, x_stride * es, cols * es, false};
-    m[n++] = {"dsum", dsum, dsum_stride * es, cols * es, false};
-    m[n++] = {"rstd", rstd, 4, 4, false};
-    m[n++] = {"the weight", weight, 0, cols * wes, false};
-    m[n++] = {"dx", dx, dx_stride * es, cols * es, true};
-    m[n++] = {"dweight", dweight, 0, cols * wes, true};
+    m[n++] = {"x", x, x_stride * es, cols * es, READ_REPLACEABLE};
+    m[n++] = {"dsum", dsum, dsum_stride * es, cols * es, READ_REPLACEABLE};
+    m[n++] = {"rstd", rstd, 4, 4, READ};
+    m[n++] = {"the weight", weight, 0, cols * wes, READ};
+    m[n++] = {"dx", dx, dx_stride * es, cols * es, WRITTEN_IN_PLACE};
+    m[n++] = {"dweight", dweight, 0, cols * wes, WRITTEN};
     if (dweight) {
       // the workspace has rows of its own: as one stretch of bytes
       const size_t bytes = alamd_rms_norm_grad_workspace(rows, cols);
-      m[n++] = {"the workspace", workspace, 0, bytes, true};
+      m[n++] = {"the workspace", workspace, 0, bytes, WRITTEN};
     }
     if ((rc = check_overlaps(m, n, rows))) return rc;
     GradParams p{};

@@ -293,7 +293,8 @@ int make_chunks(std::vector<Chunk> &table, void *const *outs, const void *const 
     if (!in || !out) return set_error(ALAMD_ERR_INVALID_ARG, "tensor %zu is null", t);
     if (!aligned_to(in, es) || !aligned_to(out, es))
       return set_error(ALAMD_ERR_INVALID_ARG, "tensor %zu is not aligned to its element type", t);
-    if (counts[t] > ((size_t)1 << 46) / es) return set_error(ALAMD_ERR_INVALID_ARG, "tensor %zu is too large", t);
+    // more than any device holds: a wrong count is refused before a table of its chunks is built
+    if (counts[t] > ((size_t)1 << 39) / es) return set_error(ALAMD_ERR_INVALID_ARG, "tensor %zu is too large", t);
     const uintptr_t at = reinterpret_cast<uintptr_t>(out);
     written.push_back({at, at + counts[t] * es, t});
     // the first chunk ends on a 64-byte boundary of the output (of the input, where they lie apart by no whole
@@ -350,7 +351,7 @@ int alamd_tensor_list_create(alamd_tensor_list **list, void *const *outs, const 
     }
     *list = made.release();
     return ALAMD_OK;
-  } catch (const std::bad_alloc &) {
+  } catch (...) {  // no C++ exception leaves a C entry
     return set_error(ALAMD_ERR_INVALID_ARG, "no host memory for a list of %zu tensors", n);
   }
 }

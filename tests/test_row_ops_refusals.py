@@ -77,6 +77,25 @@ def test_grad_refuses(lib, code, kw):
     assert lib.alamd_last_error()
 
 
+@pytest.mark.parametrize("kw", [
+    dict(out=W), dict(sum=W), dict(rstd=IN, cols=2), dict(rstd=W, cols=2), dict(scales=IN, cols=2),
+])
+def test_norm_of_one_row_replaces_rows_alone(lib, kw):
+    """A single row of a written matrix is as long as what it may not replace."""
+    assert norm(lib, rows=1, **kw) == 5
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dx=W, wdt=BF16), dict(dx=RSTD, cols=2), dict(dw=IN, wdt=BF16), dict(dw=RES, wdt=BF16), dict(dw=W), dict(dw=RSTD, cols=1),
+])
+def test_grad_of_one_row_replaces_rows_alone(lib, kw):
+    assert grad(lib, rows=1, **kw) == 5
+
+
+def test_list_refuses_more_than_a_device_holds(lib):
+    assert make(lib, [IN], [(1 << 39) // 4 + 1], [F32]) == 1
+
+
 def test_grad_of_nothing(lib):
     assert grad(lib, rows=0, dw=None) == 0
     assert grad(lib, cols=0) == 0
