@@ -189,8 +189,8 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const Chunk *table, unsi
 }
 
 // A wave for every KiB: the addresses that are under way at once stay close together, which a long list's pass is
-// faster for (2.75 GB read and written after the norm: 407 us, with a chunk of 64 KiB a workgroup 460 us, with 16 KiB
-// 450 us; fewer waves a CU than fit, as the folds like it, cost 5 to 15 %).
+// faster for (norm and clipping of 1.38 GB: 613 us, with a chunk of 64 KiB a workgroup 672 us; with LDS asked for so
+// that fewer waves fit on a CU 647 to 715 us).
 constexpr unsigned kTile = 64, kTilesPerChunk = kChunkBytes / 16 / kTile;
 template <int AUX>
 __global__ void __launch_bounds__(kTile) clip_tile_kernel(const Chunk *table, const float *norm, float max_norm, float eps) {
