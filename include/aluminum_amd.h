@@ -478,6 +478,7 @@ int alamd_rms_norm_grad(void *dx, size_t dx_stride, const void *const *dys, int 
  * mixed as they come), and where they go when they are clipped: outs[t], or in
  * place where outs is NULL or outs[t] == ins[t].  No other overlap of what is
  * written with anything is taken (ALAMD_ERR_OVERLAP): a buffer can be in a list once.
+ * A buffer of more than 512 GiB is ALAMD_ERR_INVALID_ARG.
  * A set-up call: it allocates device memory for the table and returns when that
  * is filled.  The list holds the addresses; it belongs to the current device,
  * and the buffers stay the caller's and have to outlive its use, as the list has
