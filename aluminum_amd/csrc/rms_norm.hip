@@ -367,6 +367,13 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
       }
     }
     if (p.dx) {
+      // dx may take dsum's place, and a vector that was moved back shares elements with another lane's, which that
+      // lane writes once the team has met: its own wave has dsum in registers by then (what is read of the other
+      // streams has gone into `dot`).
+      if (p.dsum && team.ragged) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) asm volatile("" : "+v"(now.ds.raw[v]));
+      }
       const float m = team.sum(dot, lds[turn]) * p.inv_n * now.rstd;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
@@ -376,7 +383,6 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
         Row<T>::unpack(x, now.x.raw[v]);
 #pragma unroll
         for (int j = 0; j < VE; ++j) g[v][j] = fmaf(-m, x[j], g[v][j]);
-        // (dsum was read before the team met: dx may take its place)
         if (p.dsum) {
           float d[VE];
           Row<T>::unpack(d, now.ds.raw[v]);

@@ -344,6 +344,20 @@ def test_backward_in_place(al, cols, place):
     assert torch.equal(t[place], dx) and torch.equal(dw, dw1)
 
 
+@pytest.mark.parametrize("dtype,cols", [("bf16", 513), ("bf16", 1025), ("f16", 4101), ("f32", 257), ("f32", 2051), ("bf16", 8193),
+                                        ("bf16", 16391), ("f32", 8194), ("f32", 16387)])
+def test_backward_in_place_where_waves_share_elements(al, dtype, cols):
+    """The last vector, moved back, is the first of a wave and shares elements with the wave's before, which writes them."""
+    import torch
+    rows = 600
+    x, dy, dsum = (_matrix((rows, cols), _torch_type(dtype), 0, 30 + k)[0] for k in range(3))
+    rstd = torch.rand(rows, device="cuda") + 0.5
+    want = torch.empty_like(x)
+    al.rms_norm_grad(want, [dy], x, rstd, dsum=dsum)
+    al.rms_norm_grad(dsum, [dy], x, rstd, dsum=dsum)
+    assert torch.equal(dsum, want)
+
+
 def test_gradients_against_differences(al):
     """sum(out * t) moved along the axes, in 64 bits, against dx and dweight of a call in fp32."""
     import torch
