@@ -147,7 +147,10 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int j = 0; j < VE; ++j) ss = fmaf(s[v][j], team.counts(v, j) ? s[v][j] : 0.0f, ss);
+      for (int j = 0; j < VE; ++j) {
+        const float x = team.counts(v, j) ? s[v][j] : 0.0f;  // both factors: an infinity times 0 is no number
+        ss = fmaf(x, x, ss);
+      }
   } else {
 #pragma unroll
     for (int v = 0; v < NV; ++v)
@@ -365,7 +368,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
       }
       if (team.ragged) {
 #pragma unroll
-        for (int j = 0; j < VE; ++j) dot = fmaf(g[v][j], team.counts(v, j) ? x[j] : 0.0f, dot);
+        for (int j = 0; j < VE; ++j) dot = team.counts(v, j) ? fmaf(g[v][j], x[j], dot) : dot;  // (0 times an infinity is no number)
       } else {
 #pragma unroll
         for (int j = 0; j < VE; ++j) dot = fmaf(g[v][j], x[j], dot);

@@ -6,6 +6,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 U32 = 2.0 ** -24
+TYPES = ("bf16", "f16", "f32")
 
 
 def _type(name):
@@ -46,3 +47,60 @@ def test_8_bits_are_the_nearest(al, dtype, rows, cols, group):
     got = out.to(torch.float64)
     bad = (got < torch.minimum(low, high)) | (got > torch.maximum(low, high))
     assert int(bad.sum()) == 0, "%d of %d are not the nearest" % (int(bad.sum()), bad.numel())
+
+
+def _shared_columns(dtype, cols):
+    """A column that the last vector, moved back to end with the row, has in common with the vector in front."""
+    ve = 16 // _type(dtype).itemsize
+    assert cols > ve and cols % ve
+    return cols - ve, cols // ve * ve - 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [9, 77, 513, 1029, 2051, 9001, 20001])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf")])
+def test_infinity_in_elements_that_two_lanes_hold(al, dtype, cols, value):
+    """rstd is 0 next to an infinity wherever it is: zeros, and 0 * inf in its own place."""
+    import torch
+    dt = _type(dtype)
+    for column in (0, *_shared_columns(dtype, cols), cols - 1):
+        for rows in (3, 700):
+            x = torch.ones(rows, cols, device="cuda").to(dt)
+            x[1, column] = value
+            out, rstd = torch.empty_like(x), torch.empty(rows, device="cuda")
+            al.rms_norm(out, [x], rstd=rstd)
+            torch.cuda.synchronize()
+            assert float(rstd[1]) == 0 and float(rstd[0]) > 0.9 and float(rstd[2]) > 0.9
+            assert bool(torch.isnan(out[1, column])) and int((out[1] == 0).sum()) == cols - 1
+            # a row of ones: 1 / sqrt(1 + 1e-6); half of the roundings of 1 / n, the product with it and the sum with eps, two
+            # of the root, one of the output
+            for row in (0, 2):
+                off = (out[row].double() - (1 + 1e-6) ** -0.5).abs()
+                assert float(off.max()) <= 4 * U32 + torch.finfo(dt).eps / 2
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [9, 77, 513, 1029, 2051, 9001, 20001])
+def test_backward_infinity_in_elements_that_two_lanes_hold(al, dtype, cols):
+    """With an infinite gradient the row's product sum is infinite, and so is dx where x is not 0: -inf where n is positive,
+    inf where it is negative, and inf - inf in its own place; where x is 0 the product of the two is no number."""
+    import torch
+    dt = _type(dtype)
+    for column in (0, *_shared_columns(dtype, cols), cols - 1):
+        for rows in (3, 700):
+            x = torch.ones(rows, cols, device="cuda").to(dt)
+            x[:, 1] = -1
+            x[:, column] = 1
+            dy = torch.full((rows, cols), 0.5, device="cuda").to(dt)
+            dy[1, column] = float("inf")
+            dx, rstd, dw = torch.empty_like(x), torch.ones(rows, device="cuda"), torch.empty(cols, device="cuda", dtype=dt)
+            ws = torch.empty(al.rms_norm_grad_workspace(rows, cols), dtype=torch.uint8, device="cuda")
+            al.rms_norm_grad(dx, [dy], x, rstd, dweight=dw, workspace=ws)
+            torch.cuda.synchronize()
+            want = torch.where(x[1] > 0, -float("inf"), float("inf"))
+            want[column] = float("nan")
+            assert torch.equal(torch.isnan(dx[1]), torch.isnan(want))
+            there = ~torch.isnan(want)
+            assert torch.equal(dx[1][there].float(), want[there])
+            assert bool(torch.isfinite(dx[0]).all()) and bool(torch.isfinite(dx[2]).all())
+            assert float(dw[column]) == float("inf") and int(torch.isfinite(dw).sum()) == cols - 1
