@@ -270,6 +270,7 @@ struct GradParams {
   float *partial;  // [workgroups][cols]: the weight's gradient from each workgroup's rows
   char *dweight;   // where a launch of one workgroup writes it to
   int dw32;        // in fp32
+  int replaces_dsum;  // dx takes dsum's place, and rows do not end with a whole vector
   unsigned long long dy_pitch, x_pitch, dsum_pitch, dx_pitch;
   unsigned long long rows;
   unsigned cols;
@@ -379,13 +380,10 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
       }
     }
     if (p.dx) {
-      // dx may take dsum's place, and a vector that was moved back shares elements with another lane's, which that
-      // lane writes once the team has met: its own wave has dsum in registers by then (what is read of the other
-      // streams has gone into `dot`).
-      if (p.dsum && team.ragged) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) asm volatile("" : "+v"(now.ds.raw[v]));
-      }
+      // Where dx takes dsum's place and a vector was moved back, the waves that hold it and the vector in front both read
+      // the elements that the two share and, once the team has met, write them: no load of dsum may be under way then.
+      // (What is read of the other streams has gone into `dot`.)
+      if (p.replaces_dsum) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       const float m = team.sum(dot, lds[turn]) * p.inv_n * now.rstd;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
@@ -845,6 +843,7 @@ int alamd_rms_norm_grad(void *dx, size_t dx_stride, const void *const *dys, int 
     p.partial = dweight ? static_cast<float *>(workspace) : nullptr;
     p.dweight = static_cast<char *>(dweight);
     p.dw32 = weight_dtype == ALAMD_F32;
+    p.replaces_dsum = dsum && dx == dsum && cols % (16 / es) != 0;
     p.dy_pitch = dy_stride * es;
     p.x_pitch = x_stride * es;
     p.dsum_pitch = dsum_stride * es;

@@ -104,3 +104,22 @@ def test_backward_infinity_in_elements_that_two_lanes_hold(al, dtype, cols):
             assert torch.equal(dx[1][there].float(), want[there])
             assert bool(torch.isfinite(dx[0]).all()) and bool(torch.isfinite(dx[2]).all())
             assert float(dw[column]) == float("inf") and int(torch.isfinite(dw).sum()) == cols - 1
+
+
+@pytest.mark.parametrize("dtype,cols", [("bf16", 513), ("f16", 1031), ("bf16", 4101), ("f32", 259), ("f32", 1025), ("f32", 4099), ("bf16", 6149),
+                                        ("f16", 8199), ("f32", 4613), ("bf16", 16389), ("f32", 16386)])
+@pytest.mark.parametrize("ranks", [1, 5])
+def test_backward_in_dsums_place_where_waves_share_elements(al, dtype, cols, ranks):
+    """The shared elements are read and written by the wave that holds the vector moved back and by the wave in front."""
+    import torch
+    rows = 1300
+    gen = torch.Generator(device="cuda").manual_seed(cols)
+    x, dsum, *dys = (torch.randn(rows, cols, device="cuda", generator=gen).to(_type(dtype)) for _ in range(ranks + 2))
+    w = torch.randn(cols, device="cuda", generator=gen)
+    rstd = torch.rand(rows, device="cuda", generator=gen) + 0.5
+    ws = torch.empty(al.rms_norm_grad_workspace(rows, cols), dtype=torch.uint8, device="cuda")
+    want, dw, dw1 = torch.empty_like(x), torch.empty_like(w), torch.empty_like(w)
+    al.rms_norm_grad(want, dys, x, rstd, weight=w, dsum=dsum, dweight=dw, workspace=ws)
+    al.rms_norm_grad(dsum, dys, x, rstd, weight=w, dsum=dsum, dweight=dw1, workspace=ws)
+    torch.cuda.synchronize()
+    assert torch.equal(dsum, want) and torch.equal(dw, dw1)
