@@ -105,6 +105,8 @@ def load():
     L.alamd_rms_norm_grad.argtypes = [vp, sz, pvp, i, sz, vp, sz, vp, sz, vp, vp, i, vp, sz, sz, i, vp, vp]
     L.alamd_tensor_list_create.argtypes = [pvp, pvp, pvp, C.POINTER(sz), C.POINTER(i), sz]
     L.alamd_tensor_list_destroy.argtypes = [vp]
+    L.alamd_tensor_list_workspace.argtypes = [vp]
+    L.alamd_tensor_list_workspace.restype = vp
     L.alamd_global_norm.argtypes = [vp, vp, vp, vp]
     L.alamd_clip_to_norm.argtypes = [vp, vp, fl, fl, vp]
     L.alamd_clip_global_norm.argtypes = [vp, vp, fl, fl, vp, vp]
@@ -533,8 +535,9 @@ def rms_norm_grad(dx, dys, x, rstd, weight=None, dsum=None, dweight=None, worksp
 
 class TensorList:
     """A list of buffers (alamd_tensor_list): the gradients `ins` of float16, bfloat16 and float32, clipped into `outs`
-    or in place.  Holds its tensors, and a workspace of its own for calls that are given none; such calls have to
-    follow one another."""
+    or in place.  Holds its tensors.  Calls that are given no workspace use the list's own and have to follow one another.
+    The table and that workspace stay until destroy(), which waits for the device, whether or not this object is dropped:
+    every list needs the call, after the last use of it and of the graphs that hold one."""
 
     WORKSPACE_BYTES = 16384
 
@@ -556,11 +559,11 @@ class TensorList:
         dtypes = (C.c_int * n)(*[DTYPES.index(_infer_dtype(t)) for t in self._keep[0]])
         _check(load().alamd_tensor_list_create(C.byref(self._h), None if outs is None else _table(self._keep[1]),
                                                _table(self._keep[0]), counts, dtypes, n))
-        self._workspace = torch.empty(self.WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+        self._own = load().alamd_tensor_list_workspace(self._h)
 
     def _space(self, workspace):
         if workspace is None:
-            return self._workspace.data_ptr()
+            return self._own
         if workspace.numel() * workspace.element_size() < self.WORKSPACE_BYTES:
             raise AlError(1, "the workspace has less than %d bytes" % self.WORKSPACE_BYTES)
         return _vector(workspace, workspace.numel(), workspace.dtype, self._dev, "workspace")
@@ -583,7 +586,7 @@ class TensorList:
 
     def destroy(self):
         if self._h:
-            h, self._h = self._h, C.c_void_p(None)
+            h, self._h, self._own = self._h, C.c_void_p(None), None
             _check(load().alamd_tensor_list_destroy(h))
 
 

@@ -33,6 +33,7 @@ struct alamd_tensor_list {
   size_t chunks;
   size_t bytes;
   alamd::Chunk *table;  // in device memory
+  void *workspace;      // behind the table
 };
 
 namespace alamd {
@@ -338,11 +339,14 @@ int alamd_tensor_list_create(alamd_tensor_list **list, void *const *outs, const 
   try {
     std::vector<Chunk> table;
     if (int rc = make_chunks(table, outs, ins, counts, dtypes, n)) return rc;
-    std::unique_ptr<alamd_tensor_list> made(new alamd_tensor_list{0, table.size(), 0, nullptr});
+    std::unique_ptr<alamd_tensor_list> made(new alamd_tensor_list{0, table.size(), 0, nullptr, nullptr});
     for (const Chunk &c : table) made->bytes += c.count * alamd_dtype_size(c.dtype);
     ALAMD_HIP(hipGetDevice(&made->device));
+    // (memory of the list's own, not of an allocator that hands it on in the order of another stream)
+    const size_t table_bytes = (table.size() * sizeof(Chunk) + 255) & ~(size_t)255;
+    ALAMD_HIP(hipMalloc(reinterpret_cast<void **>(&made->table), table_bytes + ALAMD_GLOBAL_NORM_WORKSPACE_BYTES));
+    made->workspace = reinterpret_cast<char *>(made->table) + table_bytes;
     if (!table.empty()) {
-      ALAMD_HIP(hipMalloc(reinterpret_cast<void **>(&made->table), table.size() * sizeof(Chunk)));
       const hipError_t e = hipMemcpy(made->table, table.data(), table.size() * sizeof(Chunk), hipMemcpyHostToDevice);
       if (e != hipSuccess) {
         (void)hipFree(made->table);
@@ -363,6 +367,8 @@ int alamd_tensor_list_destroy(alamd_tensor_list *list) {
   if (table) ALAMD_HIP(hipFree(table));
   return ALAMD_OK;
 }
+
+void *alamd_tensor_list_workspace(const alamd_tensor_list *list) { return list ? list->workspace : nullptr; }
 
 int alamd_global_norm(const alamd_tensor_list *list, float *norm, void *workspace, void *stream) {
   if (int rc = check_list(list)) return rc;

@@ -490,6 +490,9 @@ typedef struct alamd_tensor_list alamd_tensor_list;
 int alamd_tensor_list_create(alamd_tensor_list **list, void *const *outs, const void *const *ins,
                              const size_t *counts, const int *dtypes, size_t n);
 int alamd_tensor_list_destroy(alamd_tensor_list *list);
+/* A workspace that belongs to the list and lives as long, for calls with this list
+ * that follow one another, on whatever streams; NULL for NULL. */
+void *alamd_tensor_list_workspace(const alamd_tensor_list *list);
 
 /* *norm (fp32, device memory) = sqrt of the sum of the squares of every element
  * of the list, squared and summed in fp64 in an order that depends on the list
