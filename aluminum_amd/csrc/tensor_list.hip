@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <memory>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "alamd_rows.h"
@@ -26,6 +27,9 @@ struct Chunk {
   int dtype;
 };
 
+// Memory from `at` to `end`.
+struct Span { uintptr_t at, end; };
+
 }  // namespace alamd
 
 struct alamd_tensor_list {
@@ -34,6 +38,7 @@ struct alamd_tensor_list {
   size_t bytes;
   alamd::Chunk *table;  // in device memory
   void *workspace;      // behind the table
+  std::vector<alamd::Span> written, all;  // what the list's tensors occupy, in order and joined where they touch
 };
 
 namespace alamd {
@@ -216,6 +221,23 @@ int check_list(const alamd_tensor_list *list) {
   return ALAMD_OK;
 }
 
+// Sorted, with spans that touch or overlap joined.
+void join(std::vector<Span> &s) {
+  std::sort(s.begin(), s.end(), [](const Span &a, const Span &b) { return a.at < b.at; });
+  size_t n = 0;
+  for (const Span &x : s) {
+    if (n > 0 && x.at <= s[n - 1].end) s[n - 1].end = std::max(s[n - 1].end, x.end);
+    else s[n++] = x;
+  }
+  s.resize(n);
+}
+int check_apart(const std::vector<Span> &s, const void *p, size_t bytes, const char *name) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const auto first = std::upper_bound(s.begin(), s.end(), at, [](uintptr_t v, const Span &x) { return v < x.end; });
+  if (first != s.end() && first->at < at + bytes) return set_error(ALAMD_ERR_OVERLAP, "%s lies in a tensor of the list", name);
+  return ALAMD_OK;
+}
+
 int check_clip(const float *norm, float max_norm, float eps) {
   if (!norm || !aligned_to(norm, 4)) return set_error(ALAMD_ERR_INVALID_ARG, "norm is null or not aligned to fp32");
   if (!(max_norm >= 0.0f) || !(eps >= 0.0f)) return set_error(ALAMD_ERR_INVALID_ARG, "max_norm or eps is negative or not a number");
@@ -272,16 +294,17 @@ int launch_clip(const alamd_tensor_list *list, bool cached, const double *parts,
   return ALAMD_OK;
 }
 
-int check_workspace(const void *workspace, const float *norm) {
+int check_workspace(const alamd_tensor_list *list, const void *workspace, const float *norm) {
   if (!workspace || !aligned_to(workspace, 8))
     return set_error(ALAMD_ERR_INVALID_ARG, "the workspace is null or not aligned to 8 bytes");
   const uintptr_t w = reinterpret_cast<uintptr_t>(workspace), n = reinterpret_cast<uintptr_t>(norm);
   if (n + sizeof(float) > w && n < w + ALAMD_GLOBAL_NORM_WORKSPACE_BYTES)
     return set_error(ALAMD_ERR_OVERLAP, "the norm lies in the workspace");
-  return ALAMD_OK;
+  if (int rc = check_apart(list->all, norm, sizeof(float), "the norm")) return rc;
+  return check_apart(list->all, workspace, ALAMD_GLOBAL_NORM_WORKSPACE_BYTES, "the workspace");
 }
 
-int make_chunks(std::vector<Chunk> &table, void *const *outs, const void *const *ins, const size_t *counts, const int *dtypes,
+int make_chunks(std::vector<Chunk> &table, std::vector<Span> &taken, std::vector<Span> &all, void *const *outs, const void *const *ins, const size_t *counts, const int *dtypes,
                 size_t n) {
   std::vector<Range> written;
   for (size_t t = 0; t < n; ++t) {
@@ -313,6 +336,9 @@ int make_chunks(std::vector<Chunk> &table, void *const *outs, const void *const 
   for (size_t k = 1; k < written.size(); ++k)
     if (written[k].at < written[k - 1].end)
       return set_error(ALAMD_ERR_OVERLAP, "tensors %zu and %zu overlap", written[k - 1].tensor, written[k].tensor);
+  for (const Range &r : written) taken.push_back({r.at, r.end});
+  join(taken);
+  all = taken;
   if (!outs) return ALAMD_OK;
   for (size_t t = 0; t < n; ++t) {
     if (counts[t] == 0) continue;
@@ -321,7 +347,9 @@ int make_chunks(std::vector<Chunk> &table, void *const *outs, const void *const 
     for (; w != written.end() && w->at < end; ++w)
       if (w->tensor != t || w->at != at)
         return set_error(ALAMD_ERR_OVERLAP, "the output of tensor %zu overlaps the input of tensor %zu", w->tensor, t);
+    all.push_back({at, end});
   }
+  join(all);
   return ALAMD_OK;
 }
 
@@ -338,8 +366,10 @@ int alamd_tensor_list_create(alamd_tensor_list **list, void *const *outs, const 
   *list = nullptr;
   try {
     std::vector<Chunk> table;
-    if (int rc = make_chunks(table, outs, ins, counts, dtypes, n)) return rc;
-    std::unique_ptr<alamd_tensor_list> made(new alamd_tensor_list{0, table.size(), 0, nullptr, nullptr});
+    std::vector<Span> written, all;
+    if (int rc = make_chunks(table, written, all, outs, ins, counts, dtypes, n)) return rc;
+    std::unique_ptr<alamd_tensor_list> made(
+        new alamd_tensor_list{0, table.size(), 0, nullptr, nullptr, std::move(written), std::move(all)});
     for (const Chunk &c : table) made->bytes += c.count * alamd_dtype_size(c.dtype);
     ALAMD_HIP(hipGetDevice(&made->device));
     // (memory of the list's own, not of an allocator that hands it on in the order of another stream)
@@ -373,13 +403,14 @@ void *alamd_tensor_list_workspace(const alamd_tensor_list *list) { return list ?
 int alamd_global_norm(const alamd_tensor_list *list, float *norm, void *workspace, void *stream) {
   if (int rc = check_list(list)) return rc;
   if (int rc = check_clip(norm, 0.0f, 0.0f)) return rc;
-  if (int rc = check_workspace(workspace, norm)) return rc;
+  if (int rc = check_workspace(list, workspace, norm)) return rc;
   return launch_norm(list, false, norm, static_cast<double *>(workspace), as_stream(stream));
 }
 
 int alamd_clip_to_norm(const alamd_tensor_list *list, const float *norm, float max_norm, float eps, void *stream) {
   if (int rc = check_list(list)) return rc;
   if (int rc = check_clip(norm, max_norm, eps)) return rc;
+  if (int rc = check_apart(list->written, norm, sizeof(float), "the norm")) return rc;
   return launch_clip(list, false, nullptr, 0, const_cast<float *>(norm), max_norm, eps, as_stream(stream));
 }
 
@@ -387,7 +418,7 @@ int alamd_clip_global_norm(const alamd_tensor_list *list, float *norm, float max
                            void *stream) {
   if (int rc = check_list(list)) return rc;
   if (int rc = check_clip(norm, max_norm, eps)) return rc;
-  if (int rc = check_workspace(workspace, norm)) return rc;
+  if (int rc = check_workspace(list, workspace, norm)) return rc;
   double *parts = static_cast<double *>(workspace);
   const bool cached = list->bytes <= kCachedBytes;
   if (list->chunks == 0 || in_tiles(list)) {

@@ -498,14 +498,16 @@ void *alamd_tensor_list_workspace(const alamd_tensor_list *list);
  * of the list, squared and summed in fp64 in an order that depends on the list
  * alone; 0 for an empty list.  `workspace`: ALAMD_GLOBAL_NORM_WORKSPACE_BYTES of
  * device memory, aligned to 8 bytes, that no call running at the same time uses.
- * Neither it nor the norm is part of the list or of the other. */
+ * Neither it nor the norm may be part of the list or of the other
+ * (ALAMD_ERR_OVERLAP). */
 #define ALAMD_GLOBAL_NORM_WORKSPACE_BYTES 16384
 int alamd_global_norm(const alamd_tensor_list *list, float *norm, void *workspace, void *stream);
 
 /* outs[t] = ins[t] * factor for every buffer of the list, with
  *   factor = 1 if *norm + eps <= max_norm, else max_norm / (*norm + eps)
  * in fp32, the product rounded once.  *norm is read on the device: what
- * alamd_global_norm wrote there, or the norm over more than this list.  A norm that is
+ * alamd_global_norm wrote there, or the norm over more than this list; it may not be part
+ * of what is written (ALAMD_ERR_OVERLAP).  A norm that is
  * NaN makes everything NaN; buffers that stay in place are left alone where the factor is 1. */
 int alamd_clip_to_norm(const alamd_tensor_list *list, const float *norm, float max_norm, float eps,
                        void *stream);

@@ -42,3 +42,45 @@ def test_a_list_dropped_while_a_call_runs(al):
     # the factor: its quotient; the product
     assert bool(((t - 0.5 / want).abs() <= 4 * U32 * 0.5 / want).all()) and len(junk) == 8
     assert al.load().alamd_tensor_list_destroy(handle) == 0
+
+
+def test_a_norm_or_workspace_inside_the_list(al):
+    """Refused, with nothing written; right beside it they are taken."""
+    import torch
+    room = al.TensorList.WORKSPACE_BYTES // 4
+    flat = torch.ones(5000 + 2 * room, device="cuda")
+    ins = [flat[room:room + 2000], flat[room + 2001:room + 3000]]
+    outs = [torch.ones(2001, device="cuda")[1:], torch.ones(999, device="cuda")]
+    norm = torch.zeros(1, device="cuda")
+    part = lambda t, at, n=1: t[at:at + n]  # noqa: E731
+    here, there = al.TensorList(ins), al.TensorList(ins, outs)
+    for lst, tensors in ((here, ins), (there, ins + outs)):
+        for t in tensors:
+            for at in (0, 1, t.numel() - 1):
+                for call in (lambda: lst.global_norm(part(t, at)), lambda: lst.clip_global_norm(part(t, at), 1.0)):
+                    with pytest.raises(al.AlError) as e:
+                        call()
+                    assert e.value.code == 5
+    for at in (2, room + 1998, room + 2000, room + 2998):  # a workspace that begins, ends or lies in a tensor
+        with pytest.raises(al.AlError) as e:
+            here.global_norm(norm, workspace=part(flat, at, room))
+        assert e.value.code == 5
+    for t in outs:
+        with pytest.raises(al.AlError) as e:
+            there.clip_to_norm(part(t, 5), 1.0)
+        assert e.value.code == 5
+    with pytest.raises(al.AlError) as e:
+        here.clip_to_norm(part(ins[1], 5), 1.0)
+    assert e.value.code == 5
+    torch.cuda.synchronize()
+    assert bool((flat == 1).all()) and float(norm) == 0
+    want = math.sqrt(2999)
+    for space, at in ((part(flat, 0, room), room + 2000), (part(flat, room + 3000, room), room - 1)):
+        flat.fill_(1)
+        here.global_norm(part(flat, at), workspace=space)
+        assert abs(float(flat[at]) - want) <= 1.5 * U32 * want
+    there.clip_to_norm(part(ins[0], 5), 2.0)  # read by the call as well, and by nothing written
+    torch.cuda.synchronize()
+    assert bool((outs[0] == 1).all())
+    here.destroy()
+    there.destroy()
