@@ -555,8 +555,11 @@ class TensorList:
             for k, (a, b) in enumerate(zip(*self._keep)):
                 if a.numel() != b.numel() or a.dtype != b.dtype:
                     raise AlError(1, "output %d is not like its tensor" % k)
+        for t in self._keep[0]:
+            if t.dtype not in _TYPE_CODES:
+                raise AlError(3, "a list takes float16, bfloat16 and float32, not %s" % t.dtype)
         counts = (C.c_size_t * n)(*[t.numel() for t in self._keep[0]])
-        dtypes = (C.c_int * n)(*[DTYPES.index(_infer_dtype(t)) for t in self._keep[0]])
+        dtypes = (C.c_int * n)(*[_TYPE_CODES[t.dtype] for t in self._keep[0]])
         _check(load().alamd_tensor_list_create(C.byref(self._h), None if outs is None else _table(self._keep[1]),
                                                _table(self._keep[0]), counts, dtypes, n))
         self._own = load().alamd_tensor_list_workspace(self._h)

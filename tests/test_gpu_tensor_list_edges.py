@@ -84,3 +84,12 @@ def test_a_norm_or_workspace_inside_the_list(al):
     assert bool((outs[0] == 1).all())
     here.destroy()
     there.destroy()
+
+
+def test_types_that_the_library_does_not_know(al):
+    import torch
+    for dtype in (torch.float8_e4m3fn, torch.bool, torch.complex64, torch.float64, torch.uint8):
+        for ins in ([torch.zeros(8, dtype=dtype, device="cuda")], [torch.zeros(8, device="cuda"), torch.zeros(0, dtype=dtype, device="cuda")]):
+            with pytest.raises(al.AlError) as e:
+                al.TensorList(ins)
+            assert e.value.code == 3
