@@ -1209,6 +1209,19 @@ inline size_t halo_face_elems(const size_t dims[3], size_t halo, int face) {
   return alamd_halo_face_elems(dims, halo, face);
 }
 
+/** The ranks' pointers as a C entry takes them; no table, or a number of ranks that is out of range, is left to that
+ *  entry to refuse, which then reads none. */
+class RankTable {
+ public:
+  template <typename T> RankTable(const T *const *p, int ranks) {
+    if (p && ranks > 0 && ranks <= ALAMD_MAX_RANKS) table_.assign(p, p + ranks);
+  }
+  const void *const *get() const { return table_.empty() ? nullptr : table_.data(); }
+
+ private:
+  std::vector<const void *> table_;
+};
+
 /** Root-mean-square norm of the sum of `ranks` contributions and a residual: what follows the Allreduce of a
  *  layer's partial results, in the pass that folds them (alamd_rms_norm).  T is a 16-bit float or float, W that or
  *  float; sum, residual, weight and rstd may be null.  Strides are in elements between rows.  This and the calls
@@ -1216,8 +1229,8 @@ inline size_t halo_face_elems(const size_t dims[3], size_t halo, int face) {
 template <typename T, typename W>
 void rms_norm(T *out, size_t out_stride, T *sum, const T *residual, size_t residual_stride, const T *const *ins, int ranks,
               size_t in_stride, const W *weight, float *rstd, size_t rows, size_t cols, float eps, Communicator &comm) {
-  std::vector<const void *> tab(ins, ins + (ranks > 0 ? ranks : 0));
-  AL_AMD_CHECK(alamd_rms_norm(out, out_stride, sum, residual, residual_stride, tab.data(), ranks, in_stride, weight,
+  const RankTable tab(ins, ranks);
+  AL_AMD_CHECK(alamd_rms_norm(out, out_stride, sum, residual, residual_stride, tab.get(), ranks, in_stride, weight,
                               TypeMap<W>::value, rstd, nullptr, 0, rows, cols, TypeMap<T>::value, eps, comm.get_stream()));
 }
 /** The same to 8 bits an element (e4m3) with a scale for every `group` columns, or for every row (group = 0). */
@@ -1226,8 +1239,8 @@ void rms_norm_e4m3(uint8_t *out, size_t out_stride, float *scales, size_t group,
                    const T *const *ins, int ranks, size_t in_stride, const W *weight, float *rstd, size_t rows, size_t cols,
                    float eps, Communicator &comm) {
   if (!scales) AL_AMD_THROW("An 8-bit output needs scales");
-  std::vector<const void *> tab(ins, ins + (ranks > 0 ? ranks : 0));
-  AL_AMD_CHECK(alamd_rms_norm(out, out_stride, sum, residual, residual_stride, tab.data(), ranks, in_stride, weight,
+  const RankTable tab(ins, ranks);
+  AL_AMD_CHECK(alamd_rms_norm(out, out_stride, sum, residual, residual_stride, tab.get(), ranks, in_stride, weight,
                               TypeMap<W>::value, rstd, scales, group, rows, cols, TypeMap<T>::value, eps, comm.get_stream()));
 }
 /** Its backward pass (alamd_rms_norm_grad); `workspace`: rms_norm_grad_workspace(rows, cols) bytes of device memory. */
@@ -1236,8 +1249,8 @@ template <typename T, typename W>
 void rms_norm_grad(T *dx, size_t dx_stride, const T *const *dys, int ranks, size_t dy_stride, const T *x, size_t x_stride,
                    const T *dsum, size_t dsum_stride, const float *rstd, const W *weight, W *dweight, size_t rows, size_t cols,
                    void *workspace, Communicator &comm) {
-  std::vector<const void *> tab(dys, dys + (ranks > 0 ? ranks : 0));
-  AL_AMD_CHECK(alamd_rms_norm_grad(dx, dx_stride, tab.data(), ranks, dy_stride, x, x_stride, dsum, dsum_stride, rstd, weight,
+  const RankTable tab(dys, ranks);
+  AL_AMD_CHECK(alamd_rms_norm_grad(dx, dx_stride, tab.get(), ranks, dy_stride, x, x_stride, dsum, dsum_stride, rstd, weight,
                                    TypeMap<W>::value, dweight, rows, cols, TypeMap<T>::value, workspace, comm.get_stream()));
 }
 
