@@ -426,8 +426,9 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const GradParams
       put(d, v);
     }
   } else {
-    // the upper half of the teams hands its part to the lower half, until one team has all
-    for (unsigned n = p.shape.teams; n > 1;) {
+    // the upper half of the teams hands its part to the lower half, until one team has all (rows of two vectors a lane
+    // have one team)
+    for (unsigned n = NV == 1 ? p.shape.teams : 1; n > 1;) {
       const unsigned half = (n + 1) / 2;
       const unsigned room = NV * (VE / 4) * team.size;
       if (team.index >= half && team.index < n) {
@@ -604,7 +605,7 @@ inline bool whole_lines(const void *at, size_t pitch, size_t bytes) {
 constexpr size_t kStreamFromBytes = (size_t)256 << 20, kGradStreamFromBytes = (size_t)64 << 20;
 
 // Waves that hold a row of `need` vectors, nv of them a lane.
-inline unsigned waves_for(unsigned need, unsigned nv) { return (need + 64 * nv - 1) / (64 * nv); }
+constexpr unsigned waves_for(unsigned need, unsigned nv) { return (need + 64 * nv - 1) / (64 * nv); }
 
 // The call on the rows from the first `done` on.
 inline NormParams from_row(NormParams p, size_t done) {
@@ -666,9 +667,10 @@ template <typename T> int norm_rows(NormParams &p, int out, hipStream_t stream) 
   if (p.rows <= 512 && one <= kMaxWaves) return launch_norm<T, 1>(p, out, halves, one, 1, stream);
   if (3 * three < 2 * two && three <= kMaxWaves) return launch_norm<T, 3>(p, out, halves, three, three == 1 ? 4 : 1, stream);
   if (two <= kMaxWaves) return launch_norm<T, 2>(p, out, halves, two, two == 1 ? 4 : 1, stream);
-  if (four <= kMaxWaves) return launch_norm<T, 4>(p, out, halves, four, 1, stream);
-  if constexpr (sizeof(T) == 4) return launch_norm<T, 8>(p, out, halves, waves_for(need, 8), 1, stream);
-  return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
+  if constexpr (sizeof(T) == 4)
+    if (four > kMaxWaves) return launch_norm<T, 8>(p, out, halves, waves_for(need, 8), 1, stream);
+  static_assert(waves_for(kMaxCols / VE, sizeof(T) == 4 ? 8 : 4) <= kMaxWaves, "the longest row fits a workgroup");
+  return launch_norm<T, 4>(p, out, halves, four, 1, stream);
 }
 
 // Workgroups whose partial sums of the weight's gradient are kept: one for every CU.  (With two the parts, which grow
@@ -688,16 +690,16 @@ int launch_grad_b(GradParams &p, size_t *parts, unsigned waves, unsigned teams, 
   ALAMD_HIP(hipGetLastError());
   return ALAMD_OK;
 }
-template <typename T, int NV, int THREADS>
-int launch_grad(GradParams &p, size_t *parts, unsigned waves, hipStream_t stream) {
+// Rows of one vector a lane.
+template <typename T> int launch_grad(GradParams &p, size_t *parts, unsigned waves, hipStream_t stream) {
   // As many rows a workgroup as it has waves for, so that there are few parts to join; but every CU gets a row first,
   // except where one workgroup does the whole call in two turns, which saves the second launch.
-  unsigned teams = THREADS / 64 / waves;
+  unsigned teams = kMaxWaves / waves;
   if (!p.partial || p.rows > 2 * (size_t)teams)
     while (teams > 1 && p.rows < (size_t)256 * teams) --teams;
   if (teams > p.rows) teams = (unsigned)p.rows;
-  return p.P == 1 ? launch_grad_b<T, NV, 1, false, THREADS>(p, parts, waves, teams, stream)
-                  : launch_grad_b<T, NV, 4, false, THREADS>(p, parts, waves, teams, stream);
+  return p.P == 1 ? launch_grad_b<T, 1, 1, false, 1024>(p, parts, waves, teams, stream)
+                  : launch_grad_b<T, 1, 4, false, 1024>(p, parts, waves, teams, stream);
 }
 
 template <typename T> int grad_rows(GradParams &p, size_t *parts, hipStream_t stream) {
@@ -715,12 +717,14 @@ template <typename T> int grad_rows(GradParams &p, size_t *parts, hipStream_t st
   // One vector a lane up to 12 waves, two from there on (us, one / two: 256 rows of 4096 bf16 8.1 / 8.6, 4 ranks of 2777 x
   // 5125 f16 53.7 / 55.7, 16384 x 8192 bf16 182 / 179); rows longer than a workgroup of eight waves can read ahead in its
   // registers are read as they come.
-  if (one <= 12) return launch_grad<T, 1, 1024>(p, parts, one, stream);
-  if (two <= 8) return launch_grad<T, 2, 512>(p, parts, two, stream);
+  if (one <= 12) return launch_grad<T>(p, parts, one, stream);
+  if (two <= 8)
+    return p.P == 1 ? launch_grad_b<T, 2, 1, false, 512>(p, parts, two, 1, stream)
+                    : launch_grad_b<T, 2, 4, false, 512>(p, parts, two, 1, stream);
   if (two <= kMaxWaves) return launch_grad_b<T, 2, 1, false, 1024>(p, parts, two, 1, stream);
-  if (four <= kMaxWaves) return launch_grad_b<T, 4, 1, true, 1024>(p, parts, four, 1, stream);
-  if constexpr (sizeof(T) == 4) return launch_grad_b<T, 8, 1, true, 1024>(p, parts, waves_for(need, 8), 1, stream);
-  return set_error(ALAMD_ERR_INVALID_ARG, "too many columns");
+  if constexpr (sizeof(T) == 4)
+    if (four > kMaxWaves) return launch_grad_b<T, 8, 1, true, 1024>(p, parts, waves_for(need, 8), 1, stream);
+  return launch_grad_b<T, 4, 1, true, 1024>(p, parts, four, 1, stream);
 }
 
 }  // namespace
