@@ -93,3 +93,34 @@ def test_types_that_the_library_does_not_know(al):
             with pytest.raises(al.AlError) as e:
                 al.TensorList(ins)
             assert e.value.code == 3
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("lead,out_lead", [(0, 1), (1, 0), (1, 2), (3, 5), (2, 33), (31, 16)])
+@pytest.mark.parametrize("count", [1, 30, 40_000, 36_000_001])
+def test_outputs_that_lie_otherwise_than_their_inputs(al, dtype, lead, out_lead, count):
+    """16-bit outputs may be apart from their inputs by no whole number of dwords, and any by no whole 64 bytes; the largest
+    list is long enough to be clipped by the KiB."""
+    import torch
+    dt = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    flat = torch.randn(lead + count, device="cuda", generator=torch.Generator(device="cuda").manual_seed(count)).to(dt)
+    room = torch.full((out_lead + count + 40,), 7.0, dtype=dt, device="cuda")
+    lst = al.TensorList([flat[lead:]], [room[out_lead:out_lead + count]])
+    norm = torch.empty(1, device="cuda")
+    want = float(flat[lead:].double().square().sum().sqrt())
+    for both in (True, False):
+        room.fill_(7)
+        if both:
+            lst.clip_global_norm(norm, want / 3, eps=0.0)
+        else:
+            lst.global_norm(norm)
+            lst.clip_to_norm(norm, want / 3, eps=0.0)
+        torch.cuda.synchronize()
+        assert abs(float(norm) - want) <= 1.5 * U32 * want
+        y = flat[lead:].double() / 3
+        # max_norm as fp32, the norm, their quotient and the product in fp32; half a step of the output, or of its least number
+        info = torch.finfo(dt)
+        off = (room[out_lead:out_lead + count].double() - y).abs()
+        assert bool((off <= (info.eps / 2 + 6 * U32) * y.abs() + info.tiny * info.eps / 2).all())
+        assert bool((room[:out_lead] == 7).all()) and bool((room[out_lead + count:] == 7).all())
+    lst.destroy()
