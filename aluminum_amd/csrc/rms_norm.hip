@@ -64,17 +64,22 @@ __device__ __forceinline__ float scale_of(float amax) {
 // and the scale's.  The factor for s * w, 448 / am rounded once (a product with the approximate reciprocal, and a step of
 // Newton's iteration on what it leaves), so that a quotient is off by that rounding, its own, and that of s * w.  (Of 134
 // million of 8191 x 4099 f16, 16 go to the wrong side of a middle between two e4m3 numbers, against 40 through rstd / scale,
-// in the same time; the 1103 that lie in the middle go to either.)  A group of zeros has any factor.  Where am or rstd is out of
-// range, y takes the place of s * w and is divided by the scale.
-template <int VE> __device__ __forceinline__ float quotient_factor(float (&s)[VE], float rstd, float am, float scale) {
-  // 2^-40 and 2^60, whose order is that of their bits; am * rstd / 448 is then above 2^-126
-  constexpr uint32_t kNear = 0x2b800000u, kFar = 0x5d800000u;
+// in the same time; the 1103 that lie in the middle go to either.)  A group of zeros has any factor.  Where am or rstd is
+// out of range (2^-40 to 2^60, whose order is that of their bits; am * rstd / 448 is then above 2^-126), y is divided by
+// the scale instead.
+constexpr uint32_t kNear = 0x2b800000u, kFar = 0x5d800000u;
+__device__ __forceinline__ bool factor_in_range(float am, float rstd) {
   const uint32_t bits = __float_as_uint(am);
-  const bool in_range = ((bits == 0) | (bits - kNear <= kFar - kNear)) & (__float_as_uint(rstd) - kNear <= kFar - kNear);
-  if (__builtin_amdgcn_ballot_w64(!in_range) == 0) {
-    const float a = __uint_as_float(bits < kNear ? kNear : bits), inv = __builtin_amdgcn_rcpf(a), by = kE4m3Max * inv;
-    return fmaf(fmaf(-by, a, kE4m3Max), inv, by);
-  }
+  return ((bits == 0) | (bits - kNear <= kFar - kNear)) & (__float_as_uint(rstd) - kNear <= kFar - kNear);
+}
+__device__ __forceinline__ float factor_of(float am) {
+  const uint32_t bits = __float_as_uint(am);
+  const float a = __uint_as_float(bits < kNear ? kNear : bits), inv = __builtin_amdgcn_rcpf(a), by = kE4m3Max * inv;
+  return fmaf(fmaf(-by, a, kE4m3Max), inv, by);
+}
+// The factor for what is left in s, which is y where the wave's part of the row has a group that is out of range.
+template <int VE> __device__ __forceinline__ float quotient_factor(float (&s)[VE], float rstd, float am, float scale) {
+  if (__builtin_amdgcn_ballot_w64(!factor_in_range(am, rstd)) == 0) return factor_of(am);
 #pragma unroll
   for (int j = 0; j < VE; ++j) s[j] *= rstd;
   return __builtin_amdgcn_rcpf(scale);
@@ -230,7 +235,7 @@ template <typename T, bool E4M3>
 __global__ void __launch_bounds__(256) rms_norm_short_kernel(const NormParams p) {
   const unsigned long long row = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
   if (row < p.rows) {
-    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0}, ss = 0.0f, am = 0.0f;
+    float s[8], ss = 0.0f, am = 0.0f;
     for (unsigned c = 0; c < p.cols; ++c) {
       float x = 0.0f;
       for (int k = 0; k < p.P; ++k) {
@@ -250,10 +255,12 @@ __global__ void __launch_bounds__(256) rms_norm_short_kernel(const NormParams p)
       am = larger(am, s[c]);
     }
     if constexpr (E4M3) {
-      const float scale = scale_of(__builtin_fabsf(am * rstd)), by = quotient_factor(s, rstd, am, scale);
+      const float scale = scale_of(__builtin_fabsf(am * rstd));
+      const bool near = factor_in_range(am, rstd);  // (a wave has 64 rows here, and each keeps to itself)
+      const float by = near ? factor_of(am) : __builtin_amdgcn_rcpf(scale);
       p.scales[row] = scale;
       for (unsigned c = 0; c < p.cols; ++c)
-        p.out[row * p.out_pitch + c] = (char)(__builtin_amdgcn_cvt_pk_fp8_f32(s[c] * by, 0.0f, 0, false) & 0xff);
+        p.out[row * p.out_pitch + c] = (char)(__builtin_amdgcn_cvt_pk_fp8_f32((near ? s[c] : s[c] * rstd) * by, 0.0f, 0, false) & 0xff);
     } else {
       for (unsigned c = 0; c < p.cols; ++c) Row<T>::put(p.out + row * p.out_pitch, c, s[c] * rstd);
     }

@@ -49,6 +49,25 @@ def test_8_bits_are_the_nearest(al, dtype, rows, cols, group):
     assert int(bad.sum()) == 0, "%d of %d are not the nearest" % (int(bad.sum()), bad.numel())
 
 
+@pytest.mark.parametrize("dtype,cols", [("f16", 5), ("f32", 3), ("f16", 520)])
+def test_8_bits_of_a_row_depend_on_it_alone(al, dtype, cols):
+    """Rows whose numbers are too small for the usual way to their quotients, among others."""
+    import torch
+    rows = 9_000_000 // cols
+    gen = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.randn(rows, cols, device="cuda", generator=gen).to(_type(dtype))
+    w = (1 + 0.2 * torch.randn(cols, device="cuda", generator=gen)).to(x.dtype)
+    got = []
+    for small in (False, True):
+        if small:
+            x[::61] *= 1e-38
+        out = torch.empty(rows, cols, dtype=torch.float8_e4m3fn, device="cuda")
+        al.rms_norm(out, [x], weight=w, scales=torch.empty(rows, 1, device="cuda"))
+        got.append(out.view(torch.uint8))
+    got[0][::61] = got[1][::61]
+    assert torch.equal(*got)
+
+
 def _shared_columns(dtype, cols):
     """A column that the last vector, moved back to end with the row, has in common with the vector in front."""
     ve = 16 // _type(dtype).itemsize
