@@ -113,9 +113,11 @@ struct RowPolicy { bool stream_loads, write_through; };
 // rows of an even pitch: one stream 73 us, two 117 us; from rows of an even pitch 63 and 84).  It is read from
 // the dword it starts in instead - the two bytes before it that come along share that dword -, and `settle`
 // moves every lane's elements down by one, the last coming from the next lane, or, at the end of a wave's run,
-// from a dword that the wave reads as a scalar: 65 and 93 us.  The backward pass lets loads split dwords: it is
-// bound by its instructions there, and what the moves cost (12 a vector and stream) is what the loads gain (121 us
-// either way); with the next row's scalars under way, every meeting of a team would wait for them besides (207 us).
+// from a dword that the wave reads as a scalar: 65 and 93 us.  The backward pass lets loads split dwords, which costs it
+// a quarter (16384 rows of 5125 bf16 126 us, from inputs of an even pitch 93, dx at either): what these moves cost (12
+// a vector and stream) is what the loads gain (121 us either way), and with the next row's scalars under way every
+// meeting of a team would wait for them besides (207 us).  What needs no moves is not built: rows that lie an even
+// number apart have one parity, so that a team of odd rows could begin its vectors at the row's second element.
 template <typename T, int NV, bool HALVES> struct RowTeam {
   static_assert(!HALVES || sizeof(T) == 2, "only 16-bit elements start in the middle of a dword");
   static constexpr int VE = Row<T>::VE;
@@ -266,9 +268,10 @@ template <typename T, int NV, bool HALVES> struct RowTeam {
   }
 
   // x * by in e4m3, a byte each.  `apart`: what a vector that was moved back shares with the lane before belongs
-  // to that lane's group, whose scale is another, and is left to that lane.  (Stores of eight bytes a lane that
-  // split dwords, as in three rows of four of 4099 columns, cost little: 35 us against 32 us at 4104 columns and
-  // 8191 rows.  Whole dwords put together across lanes, with single bytes at both ends of a wave's run, took 51.)
+  // to that lane's group, whose scale is another, and is left to that lane.  (8191 rows of f16
+  // in groups of 128: 26.2 us at 4099 columns, where stores of eight bytes a lane split dwords in three rows of four, 24.8
+  // at 4104, 22.3 at 4096.  Whole dwords put together across lanes, with single bytes at both ends of a wave's run, were
+  // slower by half than such stores when both were tried, 51 us against 35.)
   __device__ __forceinline__ void store_e4m3(const float (&x)[VE], int v, float by, bool apart, char *base, unsigned long long pitch,
                                              unsigned long long row, bool live) const {
     uint32_t q[VE / 4];

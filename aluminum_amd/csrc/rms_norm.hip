@@ -21,9 +21,10 @@
 // Both passes are bound by memory from a few thousand rows on (8192 x 8192 bf16 with residual and sum: 537 MB in
 // 88 us, 6.1 TB/s, where a large copy reaches 6.5; backward pass of 16384 x 8192 with dsum: 1.07 GB in 178 us,
 // 6.0 TB/s), by the launches and one trip to memory below (one token of 8 x 4096: 3.6 us; backward pass of 64 x
-// 1024 fp32 in two launches 5.1 us), and by their instructions where little moves for an element: with 8-bit
-// outputs (8191 x 4099 f16 in groups of 128: 26 us, of which 16 are the bytes') a wave's fixed part counts, so a
-// row is not cut finer than it has to be and nothing is in a loop that need not be.
+// 1024 fp32 in two launches 5.2 us).  Where little moves for an element, what a wave does in turn counts: with 8-bit
+// outputs (8191 x 4099 f16 in groups of 128: 26 us, of which 16 are the bytes') the vector units are busy for half of
+// the time, and a wave's loads, arithmetic and stores follow one another, so a row is not cut finer than it has to be and
+// nothing is in a loop that need not be.
 #include "alamd_rows.h"
 
 namespace alamd {
@@ -665,7 +666,8 @@ template <typename T> int norm_rows(NormParams &p, int out, hipStream_t stream) 
     for (int k = 0; k < p.P; ++k) halves = halves || starts_in_a_dword(p.in[k], p.in_pitch);
   }
   // One vector a lane where there are few rows and time is a matter of the longest chain (one / two in
-  // us: 16 rows of 8192 bf16 3.1 / 3.2; 8191 rows of 5120 f16 33.5 / 29.6); otherwise two or three,
+  // us: bf16, 16 rows of 8192 3.1 / 3.2, 512 rows 6.8 / 7.1, 768 rows 10.0 / 9.2, of 5120 4.6 / 5.0 and 7.3 / 6.9; rows of
+  // 2048 would gain up to 2048 of them, 7.0 / 7.2; 8191 rows of 5120 f16 33.5 / 29.6); otherwise two or three,
   // whichever leaves fewer places of the team's waves empty, because a wave takes its time however little it holds
   // (8191 rows of f16, two / three: 4096 columns 24.0 / 24.4 us, 4099 columns 27.0 / 24.8, to 8 bits in groups of
   // 128 30.7 / 25.9; one a lane 31.9 and 37.3, four 28.8 and 31.1).
@@ -722,8 +724,9 @@ template <typename T> int grad_rows(GradParams &p, size_t *parts, hipStream_t st
   const unsigned need = (p.cols + VE - 1) / VE;
   const unsigned one = waves_for(need, 1), two = waves_for(need, 2), four = waves_for(need, 4);
   // One vector a lane up to 12 waves, two from there on (us, one / two: 256 rows of 4096 bf16 8.1 / 8.6, 4 ranks of 2777 x
-  // 5125 f16 53.7 / 55.7, 16384 x 8192 bf16 182 / 179); rows longer than a workgroup of eight waves can read ahead in its
-  // registers are read as they come.
+  // 5125 f16 53.7 / 55.7, 16384 x 8192 bf16 182 / 179; from 13 waves on fewer rows would gain from one, 256 of 8192 10.9 /
+  // 11.4, 4096 of 7168 42.4 / 43.3); rows longer than a workgroup of eight waves can read ahead in its registers are read
+  // as they come.
   if (one <= 12) return launch_grad<T>(p, parts, one, stream);
   if (two <= 8)
     return p.P == 1 ? launch_grad_b<T, 2, 1, false, 512>(p, parts, two, 1, stream)

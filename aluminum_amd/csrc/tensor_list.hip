@@ -270,7 +270,8 @@ int launch_norm(const alamd_tensor_list *list, bool cached, float *norm, double 
 // 207 MiB 108 / 117, 272 MiB 140 / 150, 1.3 GiB 747 / 687; keeping the last 64 to 224 MiB of that: 682 to 708).
 constexpr size_t kCachedBytes = (size_t)288 << 20;
 // From kTiledBytes on a list whose chunks are not small is clipped KiB by KiB, with the norm made in a launch of its own
-// (us, tiles / chunks: 30 MiB 19.2 / 17.8, 114 MiB of long tensors 78.1 / 80.5, 272 MiB 129 / 134, 1.3 GiB 613 / 672).
+// (us, tiles / chunks: 25 MiB 17.7 / 16.6, 30 MiB 19.2 / 17.8, 35 to 47 MiB the same, 73 MiB 38.1 / 38.4, 136 MiB 70.5 /
+// 74.2, 272 MiB 129 / 134, 1.3 GiB 613 / 672).
 constexpr size_t kTiledBytes = (size_t)64 << 20;
 bool in_tiles(const alamd_tensor_list *list) { return list->bytes >= kTiledBytes && list->bytes / list->chunks >= kChunkBytes / 2; }
 

@@ -416,7 +416,7 @@ int alamd_copy(void *dst, const void *src, size_t bytes, void *stream);
  *   s    = ins[0] + ins[1] + .. + ins[P-1] (+ residual)
  *   rstd = 1 / sqrt(sum(s * s) / cols + eps)
  *   out  = s * weight * rstd
- * in fp32; `out` and `sum` (s itself, the residual stream of the next layer)
+ * in fp32, with the product with the weight made first; `out` and `sum` (s itself, the residual stream of the next layer)
  * are each rounded once, to nearest.  P = 1 is the plain operator.  The fold
  * is not one of the named orders of alamd_combine: s is not rounded between
  * the ranks, so with 16-bit rows it is nearer to the sum than any of them and
@@ -440,11 +440,12 @@ int alamd_copy(void *dst, const void *src, size_t bytes, void *stream);
  * `sum` and `out` may each take the place of an input or of the residual (the
  * same address and stride, and for `out` no scales); other overlaps are
  * ALAMD_ERR_OVERLAP.  cols is at most ALAMD_RMS_NORM_MAX_COLS.  Nothing is done
- * for rows = 0 or cols = 0.  A row whose squares overflow fp32 has rstd = 0.
+ * for rows = 0 or cols = 0.  A row whose squares overflow fp32 has rstd = 0, one
+ * whose squares vanish in it and that has eps = 0 an infinite one.
  * The order of the additions depends on rows, cols, P and the types alone: the
  * same call gives the same bits every time.  (A row of 16-bit elements that
  * starts in the middle of a dword is read together with the two bytes in front
- * of it, which share that dword.) */
+ * of it or behind it that share its first or last dword.) */
 #define ALAMD_RMS_NORM_MAX_COLS 32768
 int alamd_rms_norm(void *out, size_t out_stride, void *sum, const void *residual,
                    size_t residual_stride, const void *const *ins, int P, size_t in_stride,
