@@ -434,9 +434,10 @@ int alamd_copy(void *dst, const void *src, size_t bytes, void *stream);
  *     the whole row (group = 0).  scales[row * groups + g] = max(max|y| / 448,
  *     2^-126) over the group, y as above before rounding, and out = y / scale
  *     rounded to nearest: out * scale stands for y.  The quotient is made in fp32,
- *     within 2^-21 of itself, so one that near to the middle between two e4m3
- *     numbers may become either.  An infinity in a group makes its scale infinite
- *     and itself NaN, a NaN makes the group NaN.
+ *     within 2^-21 of itself where nothing on the way to it is subnormal, so one
+ *     that near to the middle between two e4m3 numbers may become either.  An
+ *     infinity in a group makes its scale infinite and itself NaN, a NaN makes the
+ *     group NaN.
  * `sum` and `out` may each take the place of an input or of the residual (the
  * same address and stride, and for `out` no scales); other overlaps are
  * ALAMD_ERR_OVERLAP.  cols is at most ALAMD_RMS_NORM_MAX_COLS.  Nothing is done
