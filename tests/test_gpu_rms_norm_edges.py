@@ -142,3 +142,40 @@ def test_backward_in_dsums_place_where_waves_share_elements(al, dtype, cols, ran
     al.rms_norm_grad(dsum, dys, x, rstd, weight=w, dsum=dsum, dweight=dw1, workspace=ws)
     torch.cuda.synchronize()
     assert torch.equal(dsum, want) and torch.equal(dw, dw1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [3, 9, 77, 513, 1029, 4101])
+@pytest.mark.parametrize("group", [0, 32, 128])
+def test_8_bits_next_to_an_infinity(al, dtype, cols, group):
+    """In a row, y is 0 beside an infinity and no number in its place, which makes its group that; in the weight, y is infinite in
+    its place, the group's scale with it, and other elements of the group are 0."""
+    import torch
+    dt = _type(dtype)
+    size = group or cols
+    groups = -(-cols // size)
+    columns = (0, cols - 1) if cols < 9 else (0, *_shared_columns(dtype, cols), cols - 1)
+    for column in columns:
+        mine = torch.zeros(groups, dtype=torch.bool, device="cuda")
+        mine[column // size] = True
+        elements = mine.repeat_interleave(size)[:cols]
+        for rows in (3, 700):
+            for where in ("row", "weight"):
+                x, w = torch.ones(rows, cols, device="cuda").to(dt), torch.ones(cols, device="cuda").to(dt)
+                if where == "row":
+                    x[1, column] = float("inf")
+                else:
+                    w[column] = float("inf")
+                q, scales = torch.empty(rows, cols, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(rows, groups, device="cuda")
+                al.rms_norm(q, [x], weight=w, scales=scales, group=group)
+                q = q.float()
+                if where == "row":
+                    assert bool(torch.isnan(scales[1][mine]).all()) and bool((scales[1][~mine] == 2.0 ** -126).all())
+                    assert bool(torch.isnan(q[1][elements]).all()) and bool((q[1][~elements] == 0).all())
+                    assert bool((q[0] == 448).all()) and bool((q[2] == 448).all())
+                else:
+                    assert bool((scales[:, mine] == float("inf")).all()) and bool(torch.isfinite(scales[:, ~mine]).all())
+                    assert bool(torch.isnan(q[:, column]).all()) and bool((q[:, ~elements] == 448).all())
+                    elements_beside = elements.clone()
+                    elements_beside[column] = False
+                    assert bool((q[:, elements_beside] == 0).all())
