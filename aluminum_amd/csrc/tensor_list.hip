@@ -305,8 +305,8 @@ int check_workspace(const alamd_tensor_list *list, const void *workspace, const 
   return check_apart(list->all, workspace, ALAMD_GLOBAL_NORM_WORKSPACE_BYTES, "the workspace");
 }
 
-int make_chunks(std::vector<Chunk> &table, std::vector<Span> &taken, std::vector<Span> &all, void *const *outs, const void *const *ins, const size_t *counts, const int *dtypes,
-                size_t n) {
+int make_chunks(std::vector<Chunk> &table, std::vector<Span> &taken, std::vector<Span> &all, void *const *outs,
+                const void *const *ins, const size_t *counts, const int *dtypes, size_t n) {
   std::vector<Range> written;
   for (size_t t = 0; t < n; ++t) {
     if (dtypes[t] != ALAMD_F16 && dtypes[t] != ALAMD_BF16 && dtypes[t] != ALAMD_F32)
